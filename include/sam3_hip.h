@@ -402,6 +402,183 @@ enum sam3_error sam3_hip_sdpa_on_path(int path, int dtype, const void *q, const 
 				      int Sq, int Sk, int D, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* 8-bit floating point linear layers (device pointers, async on        */
+/* `stream`). No counterpart in the reference, whose only quantized     */
+/* weight format is Q8_0; these stand next to sam3_hip_matmul with Q8_0. */
+/*                                                                      */
+/* Values are e4m3 (OCP: 1 sign, 4 exponent, 3 mantissa bits, largest   */
+/* 448, 0x7F and 0xFF NaN, no infinities). A row of K values is stored  */
+/* as KB = ceil(K / 128) whole blocks of 128 bytes; the bytes past K    */
+/* are zero, and they take part in the sums, so a caller that lays rows */
+/* out itself writes zeros there. Activations have one f32 scale for    */
+/* each row and block, stored block-major [KB, rows]; weights one for   */
+/* each 128 x 128 block, [ceil(N / 128), KB]. Quantized tensors are     */
+/* 16-byte aligned, scales 4-byte aligned. Outputs must not overlap     */
+/* inputs.                                                              */
+/* ------------------------------------------------------------------ */
+
+/* x [rows, K] (F32, F16 or BF16, rows ldx elements apart, ldx >= K) -> q
+ * [rows, KB * 128] and scale [KB, rows]. The scale of a group is 2^e with
+ * the least e >= -126 for which its largest finite |x| is at most
+ * 448 * 2^e (a group without nonzero finite values: some power of two);
+ * q = e4m3(x * 2^-e), to nearest, ties to even. Infinities and NaN become
+ * NaN. Powers of two make x * 2^-e exact in f32, so the result does not
+ * depend on how it is computed. */
+enum sam3_error sam3_hip_fp8_quantize(int x_dtype, const void *x, long long ldx, int rows, int K,
+				      void *q, float *scale, void *stream);
+
+/* w [N, K] (F32, F16 or BF16, rows ldw elements apart, ldw >= K) -> q
+ * [N, KB * 128] and scale [ceil(N / 128), KB], by the same rule over
+ * blocks of 128 x 128. Once per weight. */
+enum sam3_error sam3_hip_fp8_quantize_weight(int w_dtype, const void *w, long long ldw, int N,
+					     int K, void *q, float *scale, void *stream);
+
+/* C[M,N] = A W^T (+bias) (GELU): C[m,n] = sum over blocks b of
+ * a_scale[b,m] * w_scale[n/128,b] * (sum over the block's k of
+ * a[m,k] * w[n,k]). a_scale and w_scale are any f32 values (not only
+ * powers of two). Sums, bias and GELU are f32, then one rounding to
+ * c_dtype (F32, F16 or BF16); bias [N] is of c_dtype. Rows of C are dense.
+ * flags: SAM3_HIP_BIAS | SAM3_HIP_GELU. K = 0 gives zeros (and the bias).
+ * For F16 and BF16 outputs the products of each group of 8 consecutive k
+ * are added on a grid of 2^-13 of the group's largest, what lies below cut
+ * off (the 8-bit matrix instruction's arithmetic: about 1.4e-5 of a result
+ * of normal values); for F32 outputs they are kept whole, at half the rate.
+ * Allocates nothing and can be captured into a graph. */
+enum sam3_error sam3_hip_matmul_fp8(const void *a, const float *a_scale, const void *w,
+				    const float *w_scale, int c_dtype, void *c, int M, int N,
+				    int K, const void *bias, int flags, void *stream);
+
+/* The whole layer: x [M, K] (F32, F16 or BF16, rows ldx elements apart)
+ * quantized as sam3_hip_fp8_quantize does, then sam3_hip_matmul_fp8: the
+ * same quantized values, sums in another order for few rows (which are
+ * quantized inside the product's kernel). More rows need
+ * sam3_hip_linear_fp8_work(M, N, K) bytes for the quantized copy: `work`
+ * (16-byte aligned, at least that many bytes, not used by anything else
+ * until the call's work is done) or, with work NULL, the library's device
+ * scratch of `stream`. A call with work NULL that needs some is refused
+ * (SAM3_EINVAL) while `stream` is captured: the graph would use scratch
+ * that later calls are given again. */
+enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, const void *w,
+				    const float *w_scale, int c_dtype, void *c, int M, int N,
+				    int K, const void *bias, int flags, void *work,
+				    size_t work_bytes, void *stream);
+/* Bytes of work space sam3_hip_linear_fp8 needs (0 for few rows). */
+size_t sam3_hip_linear_fp8_work(int M, int N, int K);
+
+/* ------------------------------------------------------------------ */
+/* Norm and rotation of queries and keys (device pointers, async).      */
+/* Next to the ROPE node (sam3_hip_kernel_rope: interleaved pairs of    */
+/* the whole head, tables, dense tensors) and LAYERNORM.                */
+/* ------------------------------------------------------------------ */
+#define SAM3_HIP_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1)                */
+#define SAM3_HIP_ROPE_HALF        1 /* pairs (i, i + rot / 2)            */
+
+/* One tensor of heads: element (b, s, h, d) at in + b*in_b + s*in_s +
+ * h*in_h + d (strides in elements, >= 0), written at out likewise. out may
+ * be `in` with the same strides (in place); otherwise it must not overlap
+ * any input. weight: the norm's factors [D] of the tensors' dtype, or NULL
+ * for ones. */
+struct sam3_hip_heads {
+	const void *in;
+	void       *out;
+	int         heads;
+	long long   in_b, in_s, in_h;
+	long long   out_b, out_s, out_h;
+	const void *weight;
+};
+
+/* For every head of q and k (k.heads may be 0): with norm,
+ * x = x / sqrt(mean(x^2) + eps) * weight over the D values; then the
+ * first rot values are rotated in pairs (a, b) by the angle
+ * pos * freq[i], i < rot / 2: amp * (a cos - b sin, a sin + b cos); the
+ * rest are copied. All in f32, rounded once; the angle is reduced in 64
+ * bits, so far positions keep their precision. */
+struct sam3_hip_norm_rope {
+	int dtype;            /* F32, F16 or BF16, of both tensors            */
+	int B, S, D;          /* D even, 2 to 512                            */
+	int rot;              /* even, 0 to D; 0: the norm alone              */
+	int layout;           /* SAM3_HIP_ROPE_*                              */
+	struct sam3_hip_heads q, k;
+	const int *pos;       /* position of (b, s) at pos[b*pos_b + s], or
+			       * NULL: position s                            */
+	long long pos_b;
+	const double *freq;   /* [rot / 2] radians per position, on the device */
+	float amp;            /* factor on rotated values (1: plain)          */
+	int   norm;           /* 0: rotation alone (weight and eps unused)    */
+	float eps;
+};
+enum sam3_error sam3_hip_norm_rope(const struct sam3_hip_norm_rope *p, void *stream);
+
+/* Frequencies for sam3_hip_norm_rope, computed on the host into freq[rot /
+ * 2] (host memory): theta^(-2i/rot), scaled for contexts `factor` times as
+ * long as the `trained` positions the model was trained on:
+ *   SAM3_HIP_ROPE_PLAIN   not scaled (factor and trained unused);
+ *   SAM3_HIP_ROPE_LINEAR  all divided by factor;
+ *   SAM3_HIP_ROPE_PARTS   by wavelength: pairs that turn at least `fast`
+ *     times within `trained` positions are kept, those that turn at most
+ *     `slow` times are divided by factor, with a ramp linear in the turns
+ *     between; *amp = 0.1 ln(factor) + 1.
+ * *amp is 1 for the first two. SAM3_EINVAL: rot odd or negative, theta <= 0,
+ * factor < 1, trained < 1, fast <= slow, or a NULL output. */
+#define SAM3_HIP_ROPE_PLAIN  0
+#define SAM3_HIP_ROPE_LINEAR 1
+#define SAM3_HIP_ROPE_PARTS  2
+enum sam3_error sam3_hip_rope_frequencies(int rot, double theta, int scaling, double factor,
+					  double trained, double fast, double slow,
+					  double *freq, float *amp);
+
+/* ------------------------------------------------------------------ */
+/* Cross attention (device pointers, async). sam3_hip_sdpa over strided */
+/* tensors, lengths per sequence and shared key heads: a decoder's      */
+/* queries over an encoder's keys and values.                           */
+/* ------------------------------------------------------------------ */
+
+/* out[b,s,h] = sum_j p_j v[b,j,h'] with p = softmax over j < k_len[b] of
+ * scale * q[b,s,h] . k[b,j,h'], h' = h / (H / Hkv). Element (b, s, h, d) of
+ * a tensor lies at b*x_b + s*x_s + h*x_h + d (strides in elements, >= 0;
+ * outputs must not overlap anything). Keys and values at k_len[b] and past
+ * are not read, query rows at q_len[b] and past neither read nor written
+ * (lengths are clamped to 0..Sk and 0..Sq). A row without keys, or whose
+ * scores are all -inf, gets zeros. Statistics and sums are f32; f16 and
+ * bf16 probabilities are rounded to the tensors' type for the product with
+ * v, and their sum is that of the rounded values. */
+struct sam3_hip_cross_attention {
+	int dtype;            /* F32, F16 or BF16, of all four tensors        */
+	int B, H, Hkv;        /* H a multiple of Hkv                          */
+	int Sq, Sk;
+	int D;                /* 1 to 256                                     */
+	float scale;          /* > 0, or 0 for 1 / sqrt(D)                    */
+	const void *q, *k, *v;
+	void *out;
+	long long q_b, q_s, q_h;
+	long long k_b, k_s, k_h;
+	long long v_b, v_s, v_h;
+	long long o_b, o_s, o_h;
+	const int *q_len, *k_len; /* device, [B], or NULL: Sq and Sk          */
+};
+
+/* Few query rows over many keys are shared out over workgroups whose parts
+ * are joined by a second kernel. The parts take
+ * sam3_hip_cross_attention_work(p) bytes: `work` (16-byte aligned, at
+ * least that many, not used by anything else until the call's work is
+ * done) or, with work NULL, the library's device scratch of `stream`; with
+ * neither (work NULL while `stream` is captured, or no memory) the keys
+ * are not shared out: slower, and rounded otherwise. work smaller than
+ * that is SAM3_EINVAL. */
+enum sam3_error sam3_hip_cross_attention(const struct sam3_hip_cross_attention *p, void *work,
+					 size_t work_bytes, void *stream);
+/* Work space of this call (0: none needed, or p invalid). */
+size_t sam3_hip_cross_attention_work(const struct sam3_hip_cross_attention *p);
+
+/* Which kernel a call runs (0 if p is invalid): 1 = 16-bit MFMA tiles
+ * through LDS, 2 = f32 MFMA, 3 = one wave per row (any alignment); and the
+ * call on a forced one, for tests (SAM3_EINVAL if it cannot run it). */
+int sam3_hip_cross_attention_path(const struct sam3_hip_cross_attention *p);
+enum sam3_error sam3_hip_cross_attention_on_path(int path,
+						 const struct sam3_hip_cross_attention *p,
+						 void *work, size_t work_bytes, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* Q8_0 format on the device (device pointers, async on `stream`).      */
 /* ------------------------------------------------------------------ */
 

@@ -50,6 +50,14 @@ __device__ __forceinline__ void dma16s(unsigned lds_addr, s3k_i32x4 rsrc, unsign
 		     :: "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
 }
 
+/* 4 bytes per lane into LDS at lds_addr + 4*lane (256 bytes per
+ * wave-instruction). */
+__device__ __forceinline__ void dma4s(unsigned lds_addr, s3k_i32x4 rsrc, unsigned voff)
+{
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+		     :: "s"(lds_addr), "v"(voff), "s"(rsrc) : "memory");
+}
+
 /* 32-bit LDS address of a __shared__ object. */
 __device__ __forceinline__ unsigned lds_addr_of(const void *p)
 {

@@ -426,6 +426,65 @@ const struct s3h_settings *s3h_settings(void);
  * *bytes is its size. Returns a hipError_t value. */
 int s3k_noalloc_scratch(void **ptr, size_t *bytes);
 
+/* ------------------------------------------------------------------ */
+/* e4m3 linear layers (fp8.hip): rows of ceil(K / 128) whole blocks of   */
+/* 128 bytes, scales of rows [KB, rows], of weights [ceil(N / 128), KB]  */
+/* ------------------------------------------------------------------ */
+int s3k_fp8_quantize(int kind, const void *x, long long ldx, int rows, int K, void *q,
+		     float *scale, void *stream);
+int s3k_fp8_quantize_weight(int kind, const void *w, long long ldw, int N, int K, void *q,
+			    float *scale, void *stream);
+int s3k_fp8_matmul(const void *q, const float *sa, const void *w, const float *sw, int ck,
+		   void *c, int M, int N, int K, const void *bias, int flags, void *stream);
+/* x of up to S3K_FP8_ROWS_MAX rows, quantized inside the product's kernel */
+#define S3K_FP8_ROWS_MAX 32
+int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,
+		 void *c, int M, int N, int K, const void *bias, int flags, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Norm and rotation of queries and keys (rope.hip)                      */
+/* ------------------------------------------------------------------ */
+struct s3k_heads { /* struct sam3_hip_heads */
+	const void *in;
+	void       *out;
+	int         heads;
+	long long   in_b, in_s, in_h;
+	long long   out_b, out_s, out_h;
+	const void *weight;
+};
+struct s3k_norm_rope {
+	int kind, B, S, D, rot;
+	int half;               /* pairs (i, i + rot / 2), else (2i, 2i + 1)  */
+	struct s3k_heads q, k;
+	const int *pos;
+	long long pos_b;
+	const double *freq;
+	float amp;
+	int   norm;
+	float eps;
+};
+int s3k_norm_rope(const struct s3k_norm_rope *p, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Cross attention (xattn.hip)                                           */
+/* ------------------------------------------------------------------ */
+struct s3k_xattn {
+	int kind, B, H, Hkv, Sq, Sk, D;
+	float scale;
+	const void *q, *k, *v;
+	void *out;
+	long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, o_b, o_s, o_h;
+	const int *q_len, *k_len;
+};
+enum { S3K_XATTN_MFMA = 1, S3K_XATTN_F32 = 2, S3K_XATTN_GENERIC = 3 };
+/* The kernel a call runs, and whether one can run it. */
+int s3k_xattn_path(const struct s3k_xattn *p);
+int s3k_xattn_can(const struct s3k_xattn *p, int path);
+/* Parts the keys are shared out into, and the bytes their results take */
+int s3k_xattn_parts(const struct s3k_xattn *p, int path);
+size_t s3k_xattn_bytes(const struct s3k_xattn *p, int path, int parts);
+int s3k_xattn_run(const struct s3k_xattn *p, int path, int parts, void *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

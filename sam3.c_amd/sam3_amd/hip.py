@@ -58,6 +58,19 @@ SIGNATURES = {
     "sam3_hip_matmul_q8_noalloc": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp]),
     "sam3_hip_sdpa": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "sam3_hip_sdpa_on_path": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "sam3_hip_fp8_quantize": (_i, [_i, _vp, _ll, _i, _i, _vp, _vp, _vp]),
+    "sam3_hip_fp8_quantize_weight": (_i, [_i, _vp, _ll, _i, _i, _vp, _vp, _vp]),
+    "sam3_hip_matmul_fp8": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp]),
+    "sam3_hip_linear_fp8": (_i, [_i, _vp, _ll, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _vp, _sz,
+                                 _vp]),
+    "sam3_hip_linear_fp8_work": (_sz, [_i, _i, _i]),
+    "sam3_hip_norm_rope": (_i, [_vp, _vp]),
+    "sam3_hip_rope_frequencies": (_i, [_i, C.c_double, _i, C.c_double, C.c_double, C.c_double,
+                                       C.c_double, _vp, _vp]),
+    "sam3_hip_cross_attention": (_i, [_vp, _vp, _sz, _vp]),
+    "sam3_hip_cross_attention_work": (_sz, [_vp]),
+    "sam3_hip_cross_attention_path": (_i, [_vp]),
+    "sam3_hip_cross_attention_on_path": (_i, [_i, _vp, _vp, _sz, _vp]),
     "sam3_hip_q8_quantize": (_i, [_vp, _vp, _i, _vp]),
     "sam3_hip_q8_dequantize": (_i, [_vp, _vp, _i, _vp]),
     "sam3_hip_matmul_path": (_i, [_i, _i, _i, _i, _i, _i, _i]),
@@ -85,6 +98,36 @@ SIGNATURES = {
 # kernel paths (sam3_hip_matmul_path)
 PATH_NONE, PATH_MFMA, PATH_SKINNY, PATH_GENERIC = 0, 1, 2, 3
 BIAS, GELU, B_NT = 1, 2, 4
+
+
+# layouts and scalings of sam3_hip_norm_rope / sam3_hip_rope_frequencies
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_PARTS = 0, 1, 2
+
+
+class Heads(C.Structure):
+    """struct sam3_hip_heads: Heads(in, out, heads, in strides b s h, out
+    strides b s h, weight)."""
+    _fields_ = [("inp", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int)] + \
+               [(n, C.c_longlong) for n in ("in_b", "in_s", "in_h", "out_b", "out_s", "out_h")] + \
+               [("weight", C.c_void_p)]
+
+
+class NormRope(C.Structure):
+    """struct sam3_hip_norm_rope."""
+    _fields_ = [(n, C.c_int) for n in ("dtype", "B", "S", "D", "rot", "layout")] + \
+               [("q", Heads), ("k", Heads), ("pos", C.c_void_p), ("pos_b", C.c_longlong),
+                ("freq", C.c_void_p), ("amp", C.c_float), ("norm", C.c_int), ("eps", C.c_float)]
+
+
+class CrossAttention(C.Structure):
+    """struct sam3_hip_cross_attention."""
+    _fields_ = [(n, C.c_int) for n in ("dtype", "B", "H", "Hkv", "Sq", "Sk", "D")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + \
+               [(n, C.c_longlong) for n in ("q_b", "q_s", "q_h", "k_b", "k_s", "k_h", "v_b", "v_s",
+                                            "v_h", "o_b", "o_s", "o_h")] + \
+               [("q_len", C.c_void_p), ("k_len", C.c_void_p)]
 
 
 class EvalStats(C.Structure):
@@ -251,6 +294,62 @@ def q8_batched_dev(a_dtype, a_ptr, w_ptr, c_ptr, batch, M, N, K, stride_a, strid
     check(load().sam3_hip_matmul_q8_batched(a_dtype, a_ptr, w_ptr, c_ptr, batch, M, N, K,
                                             stride_a, stride_w, stride_c, bias_ptr, flags,
                                             stream), "matmul_q8_batched")
+
+
+# ------------------------------------------- e4m3, rotation, cross attention
+def fp8_quantize_dev(dtype, x_ptr, rows, K, q_ptr, scale_ptr, ldx=None, stream=None, weight=False):
+    """sam3_hip_fp8_quantize, or with weight=True sam3_hip_fp8_quantize_weight."""
+    fn = load().sam3_hip_fp8_quantize_weight if weight else load().sam3_hip_fp8_quantize
+    check(fn(dtype, x_ptr, K if ldx is None else ldx, rows, K, q_ptr, scale_ptr, stream),
+          "fp8_quantize")
+
+
+def matmul_fp8_dev(a_ptr, a_scale_ptr, w_ptr, w_scale_ptr, c_dtype, c_ptr, M, N, K, bias_ptr=None,
+                   flags=0, stream=None):
+    check(load().sam3_hip_matmul_fp8(a_ptr, a_scale_ptr, w_ptr, w_scale_ptr, c_dtype, c_ptr, M, N,
+                                     K, bias_ptr, flags, stream), "matmul_fp8")
+
+
+def linear_fp8_work(M, N, K):
+    return load().sam3_hip_linear_fp8_work(M, N, K)
+
+
+def linear_fp8_dev(x_dtype, x_ptr, w_ptr, w_scale_ptr, c_dtype, c_ptr, M, N, K, bias_ptr=None,
+                   flags=0, ldx=None, work=None, work_bytes=0, stream=None):
+    check(load().sam3_hip_linear_fp8(x_dtype, x_ptr, K if ldx is None else ldx, w_ptr, w_scale_ptr,
+                                     c_dtype, c_ptr, M, N, K, bias_ptr, flags, work, work_bytes,
+                                     stream), "linear_fp8")
+
+
+def norm_rope_dev(dtype, B, S, D, rot, layout, q, k=None, pos=None, pos_stride=0, freq=None,
+                  amp=1.0, norm=False, eps=1e-6, stream=None):
+    """sam3_hip_norm_rope on the Heads q and k (device pointers)."""
+    p = NormRope(dtype, B, S, D, rot, layout, q, k if k is not None else Heads(), pos, pos_stride,
+                 freq, amp, int(norm), eps)
+    check(load().sam3_hip_norm_rope(C.byref(p), stream), "norm_rope")
+
+
+def rope_frequencies(rot, theta=10000.0, scaling=ROPE_PLAIN, factor=1.0, trained=1.0, fast=32.0,
+                     slow=1.0):
+    """(float64 host array [rot / 2], factor on the rotated values)."""
+    freq, amp = np.zeros(max(rot // 2, 1), np.float64), C.c_float()
+    check(load().sam3_hip_rope_frequencies(rot, theta, scaling, factor, trained, fast, slow,
+                                           freq.ctypes.data, C.byref(amp)), "rope_frequencies")
+    return freq[:rot // 2], amp.value
+
+
+def cross_attention_dev(p, work=None, work_bytes=0, stream=None, path=0):
+    """sam3_hip_cross_attention of a CrossAttention (device pointers)."""
+    lib = load()
+    if path:
+        rc = lib.sam3_hip_cross_attention_on_path(path, C.byref(p), work, work_bytes, stream)
+    else:
+        rc = lib.sam3_hip_cross_attention(C.byref(p), work, work_bytes, stream)
+    check(rc, "cross_attention")
+
+
+def cross_attention_work(p):
+    return load().sam3_hip_cross_attention_work(C.byref(p))
 
 
 def q8_quantize(x):
