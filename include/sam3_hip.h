@@ -449,20 +449,20 @@ enum sam3_error sam3_hip_matmul_fp8(const void *a, const float *a_scale, const v
 				    int K, const void *bias, int flags, void *stream);
 
 /* The whole layer: x [M, K] (F32, F16 or BF16, rows ldx elements apart)
- * quantized as sam3_hip_fp8_quantize does, then sam3_hip_matmul_fp8: the
- * same quantized values, sums in another order for few rows (which are
- * quantized inside the product's kernel). More rows need
- * sam3_hip_linear_fp8_work(M, N, K) bytes for the quantized copy: `work`
- * (16-byte aligned, at least that many bytes, not used by anything else
- * until the call's work is done) or, with work NULL, the library's device
- * scratch of `stream`. A call with work NULL that needs some is refused
- * (SAM3_EINVAL) while `stream` is captured: the graph would use scratch
- * that later calls are given again. */
+ * quantized as sam3_hip_fp8_quantize does, then sam3_hip_matmul_fp8. Up to
+ * 16 rows, 16-byte aligned and of a multiple of 8 values, are quantized
+ * inside the product's kernel: the same quantized values, sums in another
+ * order. Other calls need sam3_hip_linear_fp8_work(M, N, K) bytes for the
+ * quantized copy: `work` (16-byte aligned, at least that many bytes, not
+ * used by anything else until the call's work is done) or, with work NULL,
+ * the library's device scratch of `stream`. A call with work NULL that
+ * needs some is refused (SAM3_EINVAL) while `stream` is captured: the graph
+ * would use scratch that later calls are given again. */
 enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, const void *w,
 				    const float *w_scale, int c_dtype, void *c, int M, int N,
 				    int K, const void *bias, int flags, void *work,
 				    size_t work_bytes, void *stream);
-/* Bytes of work space sam3_hip_linear_fp8 needs (0 for few rows). */
+/* Bytes of work space sam3_hip_linear_fp8 needs at most. */
 size_t sam3_hip_linear_fp8_work(int M, int N, int K);
 
 /* ------------------------------------------------------------------ */

@@ -4,12 +4,12 @@
  *
  *   C[m,n] = sum_b sa[b,m] * sw[n/128,b] * sum_{k in b} a[m,k] * w[n,k]
  *
- * The inner sum of a block is two v_mfma_f32_32x32x64_f8f6f4 (or one
- * 16x16x128; f16 MFMAs for f32 outputs) from zero; its result times the scales is added to the f32
- * accumulators by the VALU. The product is formed transposed, with the
+ * The inner sum of a block is one v_mfma_f32_16x16x128_f8f6f4 (four f16
+ * MFMAs for f32 outputs) from zero; its result times the scales is added
+ * to the f32 accumulators by the VALU. The product is formed transposed, with the
  * weights as the MFMA's first operand: a lane then holds one row of A
- * (lane & 31), so the scale of a tile is one value per lane (sw is uniform
- * over a tile's 32 weight rows), and 4 neighbouring columns of C per
+ * (lane & 15), so the scale of a tile is one value per lane (sw is uniform
+ * over a tile's 16 weight rows), and 4 neighbouring columns of C per
  * register group, stored together. Both operands are read with the same
  * (lane, byte) -> k map, whatever it is, so the MFMA's k order is free.
  */
@@ -17,6 +17,11 @@
 #include "lds_dma.h"
 
 namespace s3k {
+
+template <int N>
+struct f8_int {
+	static constexpr int value = N;
+};
 
 typedef int f8_i8 __attribute__((ext_vector_type(8)));
 typedef int f8_i4 __attribute__((ext_vector_type(4)));
@@ -29,7 +34,7 @@ __device__ __forceinline__ f8_i8 f8_join(const uint4 &a, const uint4 &b)
 }
 
 /*
- * c + the product over 64 (32x32) or 128 (16x16) e4m3 values of k.
+ * c + the product over 128 e4m3 values of k.
  *
  * The 8-bit MFMAs add groups of 8 products (8 consecutive bytes of a lane)
  * on a grid of 2^-13 of the group's largest, cutting off what lies below
@@ -53,19 +58,6 @@ __device__ __forceinline__ s3k_f16x8 f8_widen(int lo, int hi)
 }
 
 template <bool EXACT>
-__device__ __forceinline__ s3k_f32x16 f8_mfma32(const f8_i8 &a, const f8_i8 &b, s3k_f32x16 c)
-{
-	if constexpr (EXACT) {
-#pragma unroll
-		for (int i = 0; i < 8; i += 2)
-			c = __builtin_amdgcn_mfma_f32_32x32x16_f16(f8_widen(a[i], a[i + 1]), f8_widen(b[i], b[i + 1]),
-								   c, 0, 0, 0);
-		return c;
-	} else {
-		return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-	}
-}
-template <bool EXACT>
 __device__ __forceinline__ s3k_f32x4 f8_mfma16(const f8_i8 &a, const f8_i8 &b, s3k_f32x4 c)
 {
 	if constexpr (EXACT) {
@@ -88,10 +80,9 @@ __device__ __forceinline__ int f8_exp_of(float amax)
 	return e < -126 ? -126 : e;
 }
 
-/* 2^e, -126 <= e <= 126, is pow2f(e). Four values times `down` as e4m3
- * bytes (v_cvt_pk_fp8_f32, to nearest even; |x * down| <= 448). Infinities
- * and NaN are made NaN first: what the conversion does past 448 is then
- * never asked. */
+/* Four values times `down` = 2^-e as e4m3 bytes (v_cvt_pk_fp8_f32, to
+ * nearest even; |x * down| <= 448), infinities and NaN made NaN first: what
+ * the conversion does past 448 is never asked. */
 __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float down)
 {
 	auto one = [&](float x) {
@@ -102,33 +93,200 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d,
 	return (uint32_t)w;
 }
 
-/* N values of kind at p + i, those at and past `left` zero. VEC: p + i is
- * aligned to 16 bytes and none is past the end. */
-template <int KIND, int N, bool VEC>
-__device__ __forceinline__ void f8_load(float (&x)[N], const void *p, long long i, int left)
+/* Eight values of one row as they lie in memory. */
+template <int KIND>
+struct F8Raw {
+	static constexpr int N = KIND == S3K_F32 ? 2 : 1;
+	uint4 v[N];
+};
+
+/* Values i..i+7 at p, those at and past `left` zero. vec: 16-byte aligned */
+template <int KIND>
+__device__ __forceinline__ F8Raw<KIND> f8_load8(const void *p, long long i, int left, int vec)
 {
-	if constexpr (VEC && KIND == S3K_F32) {
+	F8Raw<KIND> r;
+	if (vec && left >= 8) {
+		const uint4 *q = (const uint4 *)((const char *)p + i * (KIND == S3K_F32 ? 4 : 2));
 #pragma unroll
-		for (int j = 0; j < N / 4; ++j) {
-			const float4 t = *(const float4 *)((const float *)p + i + 4 * j);
-			x[4 * j] = t.x, x[4 * j + 1] = t.y, x[4 * j + 2] = t.z, x[4 * j + 3] = t.w;
-		}
-	} else if constexpr (VEC) {
-#pragma unroll
-		for (int j = 0; j < N / 8; ++j) {
-			const uint4 t = *(const uint4 *)((const uint16_t *)p + i + 8 * j);
-			const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-			for (int e = 0; e < 8; ++e) {
-				const uint32_t u = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
-				x[8 * j + e] = KIND == S3K_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
-			}
-		}
-	} else {
-#pragma unroll
-		for (int j = 0; j < N; ++j)
-			x[j] = j < left ? load_as_f32(p, i + j, KIND) : 0.0f;
+		for (int j = 0; j < F8Raw<KIND>::N; ++j)
+			r.v[j] = q[j];
+		return r;
 	}
+	uint32_t w[4 * F8Raw<KIND>::N];
+#pragma unroll
+	for (int j = 0; j < 4 * F8Raw<KIND>::N; ++j) {
+		w[j] = 0;
+		if constexpr (KIND == S3K_F32) {
+			if (j < left)
+				w[j] = ((const uint32_t *)p)[i + j];
+		} else {
+			if (2 * j < left)
+				w[j] = ((const uint16_t *)p)[i + 2 * j];
+			if (2 * j + 1 < left)
+				w[j] |= (uint32_t)((const uint16_t *)p)[i + 2 * j + 1] << 16;
+		}
+	}
+#pragma unroll
+	for (int j = 0; j < F8Raw<KIND>::N; ++j)
+		r.v[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+	return r;
+}
+
+/* Values i..i+7 at p, 16-byte aligned, or zeros. */
+template <int KIND>
+__device__ __forceinline__ F8Raw<KIND> f8_chunk(const void *p, long long i, bool in)
+{
+	F8Raw<KIND> r;
+#pragma unroll
+	for (int j = 0; j < F8Raw<KIND>::N; ++j)
+		r.v[j] = make_uint4(0, 0, 0, 0);
+	if (in) {
+		const uint4 *q = (const uint4 *)((const char *)p + i * (KIND == S3K_F32 ? 4 : 2));
+#pragma unroll
+		for (int j = 0; j < F8Raw<KIND>::N; ++j)
+			r.v[j] = q[j];
+	}
+	return r;
+}
+
+typedef unsigned short f8_us2 __attribute__((ext_vector_type(2)));
+
+/* The larger of two keys: magnitudes as the bits of their type without the
+ * sign, whose order is that of the values, infinities and NaN above all;
+ * 16-bit types keep two keys in a word. */
+template <int KIND>
+__device__ __forceinline__ uint32_t f8_key_max(uint32_t a, uint32_t b)
+{
+	if constexpr (KIND == S3K_F32)
+		return a > b ? a : b;
+	else
+		return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(f8_us2, a),
+									      __builtin_bit_cast(f8_us2, b)));
+}
+
+template <int KIND>
+__device__ __forceinline__ uint32_t f8_key(const F8Raw<KIND> &r)
+{
+	constexpr uint32_t MAG = KIND == S3K_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+	uint32_t k = 0;
+#pragma unroll
+	for (int j = 0; j < F8Raw<KIND>::N; ++j) {
+		k = f8_key_max<KIND>(k, f8_key_max<KIND>(r.v[j].x & MAG, r.v[j].y & MAG));
+		k = f8_key_max<KIND>(k, f8_key_max<KIND>(r.v[j].z & MAG, r.v[j].w & MAG));
+	}
+	return k;
+}
+
+/* A key as the magnitude it stands for; infinity and NaN as infinity. */
+template <int KIND>
+__device__ __forceinline__ float f8_key_value(uint32_t k)
+{
+	if constexpr (KIND == S3K_F32) {
+		return __uint_as_float(k < 0x7F800000u ? k : 0x7F800000u);
+	} else {
+		k = max(k & 0xFFFFu, k >> 16);
+		if constexpr (KIND == S3K_BF16)
+			return bf16_to_f32(k < 0x7F80u ? k : 0x7F80u);
+		else
+			return f16_to_f32(k < 0x7C00u ? k : 0x7C00u);
+	}
+}
+
+template <int KIND>
+__device__ __forceinline__ void f8_floats(const F8Raw<KIND> &r, float (&x)[8])
+{
+#pragma unroll
+	for (int e = 0; e < 8; ++e) {
+		if constexpr (KIND == S3K_F32) {
+			const uint4 &u = r.v[e / 4];
+			x[e] = __uint_as_float(e % 4 == 0 ? u.x : e % 4 == 1 ? u.y : e % 4 == 2 ? u.z : u.w);
+		} else {
+			const uint32_t u = e / 2 == 0 ? r.v[0].x : e / 2 == 1 ? r.v[0].y : e / 2 == 2 ? r.v[0].z : r.v[0].w;
+			const uint32_t b = e & 1 ? u >> 16 : u & 0xFFFFu;
+			x[e] = KIND == S3K_BF16 ? bf16_to_f32(b) : f16_to_f32(b);
+		}
+	}
+}
+
+typedef short f8_s2 __attribute__((ext_vector_type(2)));
+
+/* Eight finite values over 2^e = up as e4m3 bytes: v_cvt_scalef32_pk_fp8_*
+ * takes two values of the type as it is and the power of two, and rounds
+ * to nearest even. */
+template <int KIND>
+__device__ __forceinline__ uint2 f8_pack8(const F8Raw<KIND> &r, float up)
+{
+	f8_s2 lo = {0, 0}, hi = {0, 0};
+	if constexpr (KIND == S3K_F32) {
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, __uint_as_float(r.v[0].x), __uint_as_float(r.v[0].y), up, false);
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, __uint_as_float(r.v[0].z), __uint_as_float(r.v[0].w), up, true);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, __uint_as_float(r.v[1].x), __uint_as_float(r.v[1].y), up, false);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, __uint_as_float(r.v[1].z), __uint_as_float(r.v[1].w), up, true);
+	} else if constexpr (KIND == S3K_BF16) {
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(s3k_bf16x2, r.v[0].x), up, false);
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(s3k_bf16x2, r.v[0].y), up, true);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(s3k_bf16x2, r.v[0].z), up, false);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(s3k_bf16x2, r.v[0].w), up, true);
+	} else {
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, __builtin_bit_cast(f8_h2, r.v[0].x), up, false);
+		lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, __builtin_bit_cast(f8_h2, r.v[0].y), up, true);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hi, __builtin_bit_cast(f8_h2, r.v[0].z), up, false);
+		hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(hi, __builtin_bit_cast(f8_h2, r.v[0].w), up, true);
+	}
+	return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+/* The largest magnitude of a group of 128 values of one row, C chunks of 8
+ * in each of its lanes (the lanes that differ in the bits of LANES);
+ * infinity if it holds one or a NaN. */
+template <int KIND, int C, int LANES>
+__device__ __forceinline__ float f8_group_max(const F8Raw<KIND> (&r)[C])
+{
+	uint32_t k = 0;
+#pragma unroll
+	for (int c = 0; c < C; ++c)
+		k = f8_key_max<KIND>(k, f8_key<KIND>(r[c]));
+#pragma unroll
+	for (int m = 1; m < 64; m <<= 1)
+		if (LANES & m)
+			k = f8_key_max<KIND>(k, (uint32_t)__shfl_xor((int)k, m));
+	return f8_key_value<KIND>(k);
+}
+
+/* A group -> e4m3 bytes and the scale. Where some group of the wave holds
+ * an infinity or NaN, all of it takes the slow way. */
+template <int KIND, int C, int LANES>
+__device__ __forceinline__ float f8_group(const F8Raw<KIND> (&r)[C], uint2 (&q)[C])
+{
+	float amax = f8_group_max<KIND, C, LANES>(r);
+	if (!__any(amax > 3.402823466e38f)) {
+		const float up = pow2f(f8_exp_of(amax));
+#pragma unroll
+		for (int c = 0; c < C; ++c)
+			q[c] = f8_pack8<KIND>(r[c], up);
+		return up;
+	}
+	amax = 0.0f;
+#pragma unroll
+	for (int c = 0; c < C; ++c) {
+		float x[8];
+		f8_floats<KIND>(r[c], x);
+#pragma unroll
+		for (int e = 0; e < 8; ++e)
+			amax = fmaxf(amax, finite_abs(x[e]));
+	}
+#pragma unroll
+	for (int m = 1; m < 64; m <<= 1)
+		if (LANES & m)
+			amax = fmaxf(amax, __shfl_xor(amax, m));
+	const int e = f8_exp_of(amax);
+#pragma unroll
+	for (int c = 0; c < C; ++c) {
+		float x[8];
+		f8_floats<KIND>(r[c], x);
+		q[c] = make_uint2(f8_pack4(x[0], x[1], x[2], x[3], pow2f(-e)), f8_pack4(x[4], x[5], x[6], x[7], pow2f(-e)));
+	}
+	return pow2f(e);
 }
 
 /* ------------------------------------------------------------------ */
@@ -139,34 +297,22 @@ __device__ __forceinline__ void f8_load(float (&x)[N], const void *p, long long 
  * magnitude is a butterfly over the 16 lanes. Reads and writes are whole
  * lines; HBM bounds it.
  */
-template <int KIND, bool VEC>
+template <int KIND>
 __global__ void __launch_bounds__(256) f8_quant_rows(const void *x, long long ldx, int rows, int K,
-						      int KB, uint8_t *q, float *scale)
+						      int KB, int vec, uint8_t *q, float *scale)
 {
 	const long long g = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
 	const int li = threadIdx.x & 15;
 	if (g >= (long long)rows * KB)
 		return;
 	const int m = (int)(g / KB), kb = (int)(g - (long long)m * KB);
-	const int k0 = kb * F8_BLK + li * 8, left = K - k0;
-	float v[8];
-	if (VEC && left >= 8)
-		f8_load<KIND, 8, VEC>(v, x, m * ldx + k0, 8);
-	else
-		f8_load<KIND, 8, false>(v, x, m * ldx + k0, left);
-	float amax = 0.0f;
-#pragma unroll
-	for (int e = 0; e < 8; ++e)
-		amax = fmaxf(amax, finite_abs(v[e]));
-#pragma unroll
-	for (int off = 8; off > 0; off >>= 1)
-		amax = fmaxf(amax, __shfl_xor(amax, off));
-	const int e = f8_exp_of(amax);
-	const float down = pow2f(-e);
-	const uint32_t lo = f8_pack4(v[0], v[1], v[2], v[3], down), hi = f8_pack4(v[4], v[5], v[6], v[7], down);
-	*(uint2 *)(q + g * F8_BLK + li * 8) = make_uint2(lo, hi);
+	const int k0 = kb * F8_BLK + li * 8;
+	const F8Raw<KIND> r[1] = {f8_load8<KIND>(x, m * ldx + k0, K - k0, vec)};
+	uint2 o[1];
+	const float up = f8_group<KIND, 1, 15>(r, o);
+	*(uint2 *)(q + g * F8_BLK + li * 8) = o[0];
 	if (li == 0)
-		scale[(long long)kb * rows + m] = pow2f(e);
+		scale[(long long)kb * rows + m] = up;
 }
 
 /* Weights: a workgroup per 128 x 128 block, read twice (the second time
@@ -209,25 +355,66 @@ struct F8Args {
 	const void *bias;
 	int M, N, KB;
 	int nmt, nnt;           /* tiles along M and N                       */
-	int vec;                /* 4 columns of C (and bias) stored together */
+	int vec;                /* columns of C stored together: 1 four, 2 also
+				 * eight of 16 bits                          */
+	int bvec;               /* four values of the bias loaded together   */
+	int nr;                 /* f8_rows: weight rows of a workgroup       */
 	/* fused quantization: x in place of a, sa */
 	const void *x;
 	long long ldx;
-	int K, xvec;
+	int K;
 };
 
-/* n..n+3 of row m, already f32: bias, GELU, one rounding, stored. */
+/* The bias of columns n..n+3 (zeros without one, and past N). */
 template <int CK>
-__device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 v, int flags)
+__device__ __forceinline__ float4 f8_bias4(const F8Args &p, int n, int flags)
 {
-	float x[4] = {v.x, v.y, v.z, v.w};
+	float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+	if ((flags & S3K_EPI_BIAS) && p.bvec && n + 3 < p.N) {
+		if constexpr (CK == S3K_F32)
+			return *(const float4 *)((const float *)p.bias + n);
+		const uint2 w = *(const uint2 *)((const uint16_t *)p.bias + n);
+		if constexpr (CK == S3K_BF16)
+			return make_float4(bf16_to_f32(w.x & 0xFFFFu), bf16_to_f32(w.x >> 16),
+					   bf16_to_f32(w.y & 0xFFFFu), bf16_to_f32(w.y >> 16));
+		return make_float4(f16_to_f32(w.x & 0xFFFFu), f16_to_f32(w.x >> 16), f16_to_f32(w.y & 0xFFFFu),
+				   f16_to_f32(w.y >> 16));
+	}
+	if (flags & S3K_EPI_BIAS) {
+#pragma unroll
+		for (int e = 0; e < 4; ++e)
+			if (n + e < p.N)
+				b[e] = load_as_f32(p.bias, n + e, CK);
+	}
+	return make_float4(b[0], b[1], b[2], b[3]);
+}
+
+/* Four f32 sums: bias, GELU, rounded to 16 bits. */
+template <int CK>
+__device__ __forceinline__ uint2 f8_pack4c(const s3k_f32x4 &v, const float4 &bias, int flags)
+{
+	float x[4] = {v[0] + bias.x, v[1] + bias.y, v[2] + bias.z, v[3] + bias.w};
+	if (flags & S3K_EPI_GELU) {
+#pragma unroll
+		for (int e = 0; e < 4; ++e)
+			x[e] = gelu_tanh(x[e]);
+	}
+	if constexpr (CK == S3K_BF16)
+		return make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+	else
+		return make_uint2(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]));
+}
+
+/* Columns n..n+3 of row m, f32 sums: bias, GELU, one rounding, stored. */
+template <int CK>
+__device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 v, float4 bias, int flags)
+{
+	float x[4] = {v.x + bias.x, v.y + bias.y, v.z + bias.z, v.w + bias.w};
 	if (m >= p.M)
 		return;
+	if (flags & S3K_EPI_GELU) {
 #pragma unroll
-	for (int e = 0; e < 4; ++e) {
-		if ((flags & S3K_EPI_BIAS) && n + e < p.N)
-			x[e] += load_as_f32(p.bias, n + e, CK);
-		if (flags & S3K_EPI_GELU)
+		for (int e = 0; e < 4; ++e)
 			x[e] = gelu_tanh(x[e]);
 	}
 	const long long at = (long long)m * p.N + n;
@@ -247,202 +434,359 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
 }
 
 /*
- * Tiles of BM rows of A by BN rows of W, WM x WN waves, each BM/WM by
- * BN/WN in 32x32 MFMA tiles. A stage holds one block of 128 k of both
- * operands (rows of 8 16-byte chunks, swizzled) and the rows' scales;
- * direct-to-LDS loads fill one of two stages while the other is used.
+ * A wave's NT x MT tiles: row m + 16 j, columns n + 16 i + 4 g + 0..3 in
+ * acc[i][j] of lane group g. 16-bit outputs with whole 16-byte rows are
+ * stored 8 columns a lane: the groups' pieces of two tiles are exchanged
+ * (v_permlane32_swap, v_permlane16_swap) so that groups 0 and 1 hold the
+ * first tile and 2 and 3 the second, 64 bytes of a row together instead of
+ * 32 by halves of 8.
  */
-template <int CK, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) f8_tile(F8Args p, int flags)
+template <int CK, int NT, int MT>
+__device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (&acc)[NT][MT], int m, int n,
+					      int g, int flags)
 {
-	constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
-	constexpr int WB = BN * F8_BLK, AB = BM * F8_BLK, SB = BM * 4, STAGE = WB + AB + SB;
+	if constexpr (CK != S3K_F32 && NT % 2 == 0) {
+		if (p.vec == 2 && n + 16 * NT <= p.N) {
+#pragma unroll
+			for (int i = 0; i < NT; i += 2) {
+				const float4 b0 = f8_bias4<CK>(p, n + 16 * i + 4 * g, flags);
+				const float4 b1 = f8_bias4<CK>(p, n + 16 * i + 16 + 4 * g, flags);
+#pragma unroll
+				for (int j = 0; j < MT; ++j) {
+					const uint2 t0 = f8_pack4c<CK>(acc[i][j], b0, flags);
+					const uint2 t1 = f8_pack4c<CK>(acc[i + 1][j], b1, flags);
+					uint32_t w[4];
+#pragma unroll
+					for (int e = 0; e < 2; ++e) {
+						const auto h = __builtin_amdgcn_permlane32_swap(e ? t0.y : t0.x, e ? t1.y : t1.x,
+												false, false);
+						const auto q = __builtin_amdgcn_permlane16_swap(h[0], h[1], false, false);
+						w[e] = q[0], w[2 + e] = q[1];
+					}
+					const s3k_u32x4 v = {w[0], w[1], w[2], w[3]};
+					if (m + 16 * j < p.M)
+						__builtin_nontemporal_store(v, (s3k_u32x4 *)((uint16_t *)p.c + (long long)(m + 16 * j) * p.N +
+											      n + 16 * i + 8 * g));
+				}
+			}
+			return;
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < NT; ++i) {
+		const float4 bias = f8_bias4<CK>(p, n + 16 * i + 4 * g, flags);
+#pragma unroll
+		for (int j = 0; j < MT; ++j)
+			f8_store4<CK>(p, m + 16 * j, n + 16 * i + 4 * g,
+				      make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]), bias, flags);
+	}
+}
+
+/* Chunk c of tile row r lies at c ^ f8_swz(r). A 16-byte LDS read takes 16
+ * lanes at a time (0-3, 12-15, 20-27, then the rest of 32, then the same of
+ * the upper half); with rows of 128 bytes, row l & 15 and chunk l >> 4 (+ 4)
+ * the 16 lanes then meet all 64 banks once. */
+__device__ __forceinline__ int f8_swz(int row)
+{
+	return (row >> 1) & 7;
+}
+
+constexpr unsigned F8_STRIP = 8;
+
+/* workgroup -> tile: workgroups go to the 8 XCDs round-robin; each XCD gets
+ * a run of the tiles, taken in strips of 8 columns row by row, so that
+ * the tiles it works on share rows of A and of W in its L2 */
+__device__ __forceinline__ void f8_place(const F8Args &p, unsigned id, int &mt, int &nt)
+{
+	const unsigned total = (unsigned)p.nmt * (unsigned)p.nnt, x = id & 7u, each = total / 8u, more = total % 8u;
+	const unsigned t = x * each + (x < more ? x : more) + (id >> 3);
+	const unsigned strip = t / (F8_STRIP * (unsigned)p.nmt), in = t - strip * F8_STRIP * (unsigned)p.nmt;
+	const unsigned wide = min(F8_STRIP, (unsigned)p.nnt - strip * F8_STRIP);
+	mt = (int)(in / wide);
+	nt = (int)(strip * F8_STRIP + in % wide);
+}
+
+/*
+ * Tiles of BM rows of A by BN rows of W, WM x WN waves, each BM/WM by
+ * BN/WN in 16x16 MFMA tiles of a whole block of 128 k. A stage holds one
+ * block of both operands (rows of 8 16-byte chunks, swizzled) and the
+ * rows' scales; two stages in a ring, filled by direct-to-LDS loads a
+ * block ahead. KS such groups of waves, each with stages of its own, take
+ * every KS-th block and are added up in LDS: for few tiles, whose blocks
+ * one after the other would leave most CUs idle.
+ */
+template <int CK, int BM, int BN, int WM, int WN, int KS>
+__global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) f8_tile(F8Args p, int flags)
+{
+	constexpr int NST = 2, NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+	constexpr int WB = BN * F8_BLK, AB = BM * F8_BLK, SB = NW * 256, STAGE = WB + AB + SB;
 	constexpr int WI = BN / 8, AI = BM / 8; /* 1 KiB loads per stage */
-	static_assert((WI + AI) % NW == 0 && BN / WN <= F8_BLK && BM % 64 == 0 && BM / 64 <= NW, "tile");
-	__shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
-	const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
-	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	static_assert((WI + AI) % NW == 0 && BN / WN <= F8_BLK && BM * 4 <= SB, "tile");
+	static_assert((KS - 1) * BM * BN * 4 <= KS * NST * STAGE, "sums fit the stages");
+	__shared__ __attribute__((aligned(1024))) char smem_all[KS * NST * STAGE];
+	const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+	const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int ks = all / NW, wave = all % NW;
 	const int wm = wave % WM, wn = wave / WM;
+	char *const smem = smem_all + ks * NST * STAGE;
 	const unsigned lds0 = lds_addr_of(smem);
 
-	const int nt = (int)(blockIdx.x % (unsigned)p.nnt), mt = (int)(blockIdx.x / (unsigned)p.nnt);
-	const int n0 = nt * BN, m0 = mt * BM;
+	int n0, m0;
+	f8_place(p, blockIdx.x, m0, n0);
+	m0 *= BM, n0 *= BN;
 	const unsigned Kp = (unsigned)p.KB * F8_BLK;
 	const int wrows = min(BN, p.N - n0), arows = min(BM, p.M - m0);
 	const s3k_i32x4 rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)wrows * Kp);
 	const s3k_i32x4 ra = buf_rsrc(p.a + (long long)m0 * Kp, (unsigned)arows * Kp);
 
 	/* load j = wave + t * NW: rows 8 j .. 8 j + 7 of W, then of A; rows
-	 * past the end lie past the buffer and read as zeros */
+	 * past the end lie past the buffer and read as zeros, and so are
+	 * blocks past the last */
 	constexpr int PER = (WI + AI) / NW;
 	unsigned off[PER];
 #pragma unroll
 	for (int t = 0; t < PER; ++t) {
 		const int j = wave + t * NW;
 		const int row = (j < WI ? j : j - WI) * 8 + (lane >> 3);
-		off[t] = (unsigned)row * Kp + (unsigned)(((lane & 7) ^ lds_swz<8>(row)) * 16);
+		off[t] = (unsigned)row * Kp + (unsigned)(((lane & 7) ^ f8_swz(row)) * 16);
 	}
 	auto issue = [&](int kb, unsigned slot) {
+		const bool in = kb < p.KB;
 #pragma unroll
 		for (int t = 0; t < PER; ++t) {
 			const int j = wave + t * NW;
-			dma16s(lds0 + slot + j * 1024, j < WI ? rw : ra, off[t], (unsigned)kb * F8_BLK);
+			dma16s(lds0 + slot + j * 1024, j < WI ? rw : ra, in ? off[t] : S3K_OOB, in ? (unsigned)kb * F8_BLK : 0u);
 		}
-		if (wave < BM / 64) {
-			const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, (unsigned)arows * 4);
-			dma4s(lds0 + slot + WB + AB + wave * 256, rs, (unsigned)(wave * 256 + lane * 4));
-		}
+		const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, in ? (unsigned)arows * 4 : 0u);
+		dma4s(lds0 + slot + WB + AB + wave * 256, rs, (unsigned)(wave * 256 + lane * 4));
 	};
 
-	s3k_f32x16 acc[NT][MT];
+	s3k_f32x4 acc[NT][MT];
 #pragma unroll
 	for (int i = 0; i < NT; ++i)
 #pragma unroll
 		for (int j = 0; j < MT; ++j)
-#pragma unroll
-			for (int r = 0; r < 16; ++r)
-				acc[i][j][r] = 0.0f;
+			acc[i][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-	/* operand rows of this lane: chunk 2 c + h of row base + l32 */
-	auto frag = [&](unsigned at, int row, int s) {
-		const int z = lds_swz<8>(row);
-		const unsigned b = at + (unsigned)row * F8_BLK;
-		return f8_join(lds_rd16(b, (unsigned)(((4 * s + h) ^ z) << 4)),
-			       lds_rd16(b, (unsigned)(((4 * s + 2 + h) ^ z) << 4)));
-	};
+	/* operand row l16 of tile t: chunks g and g + 4 (the swizzle of rows 16
+	 * apart is the same) */
+	const unsigned o0 = (unsigned)(l16 * F8_BLK + ((g ^ f8_swz(l16)) << 4));
+	const unsigned o1 = (unsigned)(l16 * F8_BLK + (((g + 4) ^ f8_swz(l16)) << 4));
+	const unsigned wo = lds0 + wn * (BN / WN) * F8_BLK, ao = lds0 + WB + wm * (BM / WM) * F8_BLK;
 	const float *swp = p.sw + (long long)((n0 + wn * (BN / WN)) / F8_BLK) * p.KB;
+	const bool live = n0 + wn * (BN / WN) < p.N;
 
-	if (p.KB)
-		issue(0, 0);
-	for (int kb = 0; kb < p.KB; ++kb) {
-		const unsigned slot = (unsigned)(kb & 1) * STAGE;
+	issue(ks, 0);
+	unsigned slot = 0;
+	for (int k0 = 0; k0 < p.KB; k0 += KS) {
+		const int kb = k0 + ks;
+		/* block kb has landed here, and everywhere past the barrier; every
+		 * wave is past the block before, whose stage is filled again */
 		wait_vm<0>();
-		__syncthreads();
-		if (kb + 1 < p.KB)
-			issue(kb + 1, STAGE - slot);
-		const unsigned wat = lds0 + slot, aat = wat + WB;
-		const float sw = n0 + wn * (BN / WN) < p.N ? swp[kb] : 0.0f;
-		f8_i8 fa[MT][2];
+		wg_barrier();
+		issue(kb + KS, STAGE - slot);
+		const float sw = live && kb < p.KB ? swp[kb] : 0.0f;
+		const unsigned wat = wo + slot, aat = ao + slot;
+		f8_i8 fa[MT];
 		float s[MT];
 #pragma unroll
 		for (int j = 0; j < MT; ++j) {
-			const int row = wm * (BM / WM) + 32 * j + l32;
-			fa[j][0] = frag(aat, row, 0);
-			fa[j][1] = frag(aat, row, 1);
-			s[j] = *(const float *)(smem + slot + WB + AB + row * 4) * sw;
+			fa[j] = f8_join(lds_rd16(aat + o0, j * 16 * F8_BLK), lds_rd16(aat + o1, j * 16 * F8_BLK));
+			s[j] = *(const float *)(smem + slot + WB + AB + (wm * (BM / WM) + 16 * j + l16) * 4) * sw;
 		}
+		/* the results of tile row i are added while row i + 1 is formed */
+		s3k_f32x4 z[2][MT];
+		auto add = [&](int i) {
+#pragma unroll
+			for (int j = 0; j < MT; ++j)
+#pragma unroll
+				for (int r = 0; r < 4; ++r)
+					acc[i][j][r] = fmaf(z[i & 1][j][r], s[j], acc[i][j][r]);
+		};
 #pragma unroll
 		for (int i = 0; i < NT; ++i) {
-			const int row = wn * (BN / WN) + 32 * i + l32;
-			const f8_i8 f0 = frag(wat, row, 0), f1 = frag(wat, row, 1);
+			const f8_i8 fw = f8_join(lds_rd16(wat + o0, i * 16 * F8_BLK), lds_rd16(wat + o1, i * 16 * F8_BLK));
 #pragma unroll
-			for (int j = 0; j < MT; ++j) {
-				s3k_f32x16 z;
-#pragma unroll
-				for (int r = 0; r < 16; ++r)
-					z[r] = 0.0f;
-				z = f8_mfma32<CK == S3K_F32>(f0, fa[j][0], z);
-				z = f8_mfma32<CK == S3K_F32>(f1, fa[j][1], z);
-#pragma unroll
-				for (int r = 0; r < 16; ++r)
-					acc[i][j][r] = fmaf(z[r], s[j], acc[i][j][r]);
-			}
+			for (int j = 0; j < MT; ++j)
+				z[i & 1][j] = f8_mfma16<CK == S3K_F32>(fw, fa[j], (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f});
+			if (i > 0)
+				add(i - 1);
 		}
+		add(NT - 1);
+		slot = STAGE - slot;
 	}
+	wait_vm<0>(); /* the last stage asked for, all zeros */
+	if constexpr (KS > 1) {
+		wg_barrier();
+		float *const sum = (float *)smem_all + wave * (NT * MT * 256) + lane * 4;
+		if (ks > 0) {
+			float *const mine = sum + (ks - 1) * (BM * BN);
 #pragma unroll
-	for (int j = 0; j < MT; ++j)
+			for (int i = 0; i < NT; ++i)
 #pragma unroll
-		for (int i = 0; i < NT; ++i)
+				for (int j = 0; j < MT; ++j)
+					*(s3k_f32x4 *)(mine + (i * MT + j) * 256) = acc[i][j];
+		}
+		__syncthreads();
+		if (ks > 0)
+			return;
 #pragma unroll
-			for (int g = 0; g < 4; ++g)
-				f8_store4<CK>(p, m0 + wm * (BM / WM) + 32 * j + l32,
-					      n0 + wn * (BN / WN) + 32 * i + 8 * g + 4 * h,
-					      make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1],
-							  acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]),
-					      flags);
+		for (int o = 0; o < KS - 1; ++o)
+#pragma unroll
+			for (int i = 0; i < NT; ++i)
+#pragma unroll
+				for (int j = 0; j < MT; ++j) {
+					const s3k_f32x4 v = *(const s3k_f32x4 *)(sum + o * (BM * BN) + (i * MT + j) * 256);
+#pragma unroll
+					for (int r = 0; r < 4; ++r)
+						acc[i][j][r] += v[r];
+				}
+	}
+	f8_tile_store<CK, NT, MT>(p, acc, m0 + wm * (BM / WM) + l16, n0 + wn * (BN / WN), g, flags);
 }
 
 /*
- * Few rows (M <= 16 MT): a workgroup takes 16 weight rows and all rows of
- * x; its 8 waves share out the blocks of k (wave w takes w, w + 8, ...)
- * and add up in LDS. x is quantized in registers on the way: a lane holds
- * 32 values of row lane & 15, the group's other three quarters are in
- * lanes 16, 32 and 48 apart. The weights are read once, straight into
- * registers; they bound it, or the launch.
+ * Few rows: a workgroup takes 16 (p.nr) weight rows and 16 MT rows of A;
+ * its NWV waves share out the blocks of k (wave w takes w, w + NWV, ...)
+ * and add up in LDS. Every wave has two blocks under way in LDS of its own
+ * and meets the others only at the end. The operands come by direct-to-LDS
+ * loads, eight lanes to a row's 128 bytes: straight into registers, as the
+ * MFMA wants them, neighbouring lanes read different rows and a load takes
+ * 64 cycles of address work (17 x 1024 x 4096: 5.9 us). Latency and, with
+ * long weights, HBM bound it.
+ *
+ * XK >= 0 (MT = 1): x of that type is quantized in registers on the way: a
+ * lane holds 32 values of row lane & 15, the group's other three quarters
+ * are 16, 32 and 48 lanes on. Every workgroup repeats that, which one
+ * launch less pays for up to 16 rows; x has to be 16-byte aligned and K a
+ * multiple of 8 (the checks of other cases cost more in instruction fetches
+ * than the launch). XK < 0: quantized rows, 16 MT of
+ * them from blockIdx.y on.
  */
-template <int XK, int CK, int MT>
-__global__ void __launch_bounds__(512) f8_rows(F8Args p, int flags)
+template <int XK, int CK, int MT, int NWV>
+__global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 {
-	__shared__ float red[8][MT][256];
+	static_assert(XK < 0 || MT == 1, "quantized on the way: 16 rows");
+	constexpr int RT = XK < 0 ? 1 + MT : 1, SLOT = RT * 2048; /* row tiles of a block */
+	constexpr int RED = NWV * MT * 1024, RING = NWV * 2 * SLOT;
+	__shared__ __attribute__((aligned(1024))) char smem[RED > RING ? RED : RING];
+	float (*const red)[MT][256] = (float (*)[MT][256])smem;
 	const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const int n0 = (int)blockIdx.x * 16;
-	const long long Kp = (long long)p.KB * F8_BLK;
-	const bool live = n0 + l16 < p.N;
-	const uint8_t *wr = p.w + (long long)(n0 + l16) * Kp + 32 * g;
+	const int n0 = (int)blockIdx.x * p.nr, m0 = (int)blockIdx.y * 16 * MT;
+	const unsigned Kp = (unsigned)p.KB * F8_BLK;
+	const s3k_i32x4 rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)min(p.nr, p.N - n0) * Kp);
+	const s3k_i32x4 ra = buf_rsrc(XK < 0 ? p.a + (long long)m0 * Kp : nullptr,
+				      XK < 0 ? (unsigned)min(16 * MT, p.M - m0) * Kp : 0u);
 	const float *swp = p.sw + (long long)(n0 / F8_BLK) * p.KB;
+	const unsigned mine = lds_addr_of(smem) + wave * 2 * SLOT;
 
 	s3k_f32x4 acc[MT];
 #pragma unroll
 	for (int j = 0; j < MT; ++j)
 		acc[j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-	for (int kb = wave; kb < p.KB; kb += 8) {
-		uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
-		if (live) {
-			w0 = *(const uint4 *)(wr + (long long)kb * F8_BLK);
-			w1 = *(const uint4 *)(wr + (long long)kb * F8_BLK + 16);
+	/* rows 8 i + (lane >> 3) of a tile by load i; the swizzles of rows 8
+	 * apart differ in bit 2 */
+	const unsigned row = (unsigned)lane >> 3;
+	const unsigned off0 = row * Kp + ((lane & 7) ^ f8_swz((int)row)) * 16u;
+	const unsigned off1 = (row + 8) * Kp + ((lane & 7) ^ f8_swz((int)row + 8)) * 16u;
+	const unsigned rd0 = (unsigned)(l16 * F8_BLK + ((g ^ f8_swz(l16)) << 4));
+	const unsigned rd1 = (unsigned)(l16 * F8_BLK + (((g + 4) ^ f8_swz(l16)) << 4));
+
+	constexpr int NA = XK < 0 ? MT : 1, NX = XK < 0 ? 1 : 4;
+	float sa[2][NA], sw[2];
+	F8Raw<XK < 0 ? S3K_BF16 : XK> x[2][NX];
+	auto load = [&](auto slot, int kb) __attribute__((always_inline)) {
+		constexpr int S = decltype(slot)::value;
+		const unsigned at = mine + S * SLOT;
+		const unsigned ko = (unsigned)__builtin_amdgcn_readfirstlane(kb * F8_BLK);
+		dma16s(at, rw, off0, ko);
+		dma16s(at + 1024, rw, off1, ko);
+		sw[S] = swp[kb];
+		if constexpr (XK < 0) {
+#pragma unroll
+			for (int j = 0; j < MT; ++j) {
+				dma16s(at + 2048 + j * 2048, ra, off0 + 16 * j * Kp, ko);
+				dma16s(at + 3072 + j * 2048, ra, off1 + 16 * j * Kp, ko);
+				const int m = m0 + 16 * j + l16;
+				sa[S][j] = m < p.M ? p.sa[(long long)kb * p.M + m] : 0.0f;
+			}
+		} else {
+			const int k0 = kb * F8_BLK + 16 * g;
+#pragma unroll
+			for (int c = 0; c < 4; ++c) {
+				/* bytes 16 g and 64 + 16 g onward, as the weights' */
+				const int k = k0 + 64 * (c >> 1) + 8 * (c & 1);
+				x[S][c] = f8_chunk<XK>(p.x, l16 * p.ldx + k, l16 < p.M && k < p.K);
+			}
 		}
-		const f8_i8 fw = f8_join(w0, w1);
-		const float sw = swp[kb];
-		const int k0 = kb * F8_BLK + 32 * g;
+	};
+	auto work = [&](auto slot) __attribute__((always_inline)) {
+		constexpr int S = decltype(slot)::value;
+		const unsigned at = mine + S * SLOT;
+		const f8_i8 fw = f8_join(lds_rd16(at + rd0, 0), lds_rd16(at + rd1, 0));
 #pragma unroll
 		for (int j = 0; j < MT; ++j) {
-			const int m = 16 * j + l16;
-			float v[32];
-			if (m < p.M) {
-				if (p.xvec && k0 + 32 <= p.K)
-					f8_load<XK, 32, true>(v, p.x, m * p.ldx + k0, 32);
-				else
-					f8_load<XK, 32, false>(v, p.x, m * p.ldx + k0, p.K - k0);
-			} else {
-#pragma unroll
-				for (int e = 0; e < 32; ++e)
-					v[e] = 0.0f;
-			}
-			float amax = 0.0f;
-#pragma unroll
-			for (int e = 0; e < 32; ++e)
-				amax = fmaxf(amax, finite_abs(v[e]));
-			amax = fmaxf(amax, __shfl_xor(amax, 16));
-			amax = fmaxf(amax, __shfl_xor(amax, 32));
-			const int e = f8_exp_of(amax);
-			const float down = pow2f(-e);
 			f8_i8 fx;
+			float s;
+			if constexpr (XK < 0) {
+				fx = f8_join(lds_rd16(at + rd0, 2048 + 2048 * j), lds_rd16(at + rd1, 2048 + 2048 * j));
+				s = sa[S][j] * sw[S];
+			} else {
+				/* an infinity or NaN makes all of its row's results NaN,
+				 * whatever the group's other values become */
+				const float amax = f8_group_max<XK, 4, 48>(x[S]);
+				const float up = pow2f(f8_exp_of(amax));
+				uint2 q[4];
 #pragma unroll
-			for (int i = 0; i < 8; ++i)
-				fx[i] = (int)f8_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], down);
+				for (int c = 0; c < 4; ++c)
+					q[c] = f8_pack8<XK>(x[S][c], up);
+				s = amax <= 3.402823466e38f ? up * sw[S] : __builtin_nanf("");
+				fx = (f8_i8){(int)q[0].x, (int)q[0].y, (int)q[1].x, (int)q[1].y,
+					     (int)q[2].x, (int)q[2].y, (int)q[3].x, (int)q[3].y};
+			}
 			const s3k_f32x4 z = f8_mfma16<CK == S3K_F32>(fw, fx, (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f});
-			const float s = pow2f(e) * sw;
 #pragma unroll
 			for (int r = 0; r < 4; ++r)
 				acc[j][r] = fmaf(z[r], s, acc[j][r]);
 		}
+	};
+	f8_int<0> even;
+	f8_int<1> odd;
+	if (wave < p.KB)
+		load(even, wave);
+	if (wave + NWV < p.KB)
+		load(odd, wave + NWV);
+	for (int kb = wave; kb < p.KB; kb += 2 * NWV) {
+		wait_vm<0>(); /* both blocks: the compiler does not see these loads */
+		__builtin_amdgcn_sched_barrier(0);
+		work(even);
+		if (kb + NWV < p.KB)
+			work(odd);
+		if (kb + 2 * NWV < p.KB) {
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); /* the slots are read */
+			load(even, kb + 2 * NWV);
+			if (kb + 3 * NWV < p.KB)
+				load(odd, kb + 3 * NWV);
+		}
 	}
+	__syncthreads(); /* the sums go over the ring */
 #pragma unroll
 	for (int j = 0; j < MT; ++j)
 		*(s3k_f32x4 *)&red[wave][j][lane * 4] = acc[j];
 	__syncthreads();
 	/* thread t < 64 MT: lane t % 64 of tile t / 64, its four columns */
 	const int t = threadIdx.x;
-	if (t < 64 * MT) {
+	if (t < 64 * MT && 4 * ((t & 63) >> 4) < p.nr) {
 		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-		for (int w = 0; w < 8; ++w) {
+		for (int w = 0; w < NWV; ++w) {
 			const float4 u = *(const float4 *)&red[w][t >> 6][(t & 63) * 4];
 			v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
 		}
-		f8_store4<CK>(p, 16 * (t >> 6) + (t & 15), n0 + 4 * ((t & 63) >> 4), v, flags);
+		const int n = n0 + 4 * ((t & 63) >> 4);
+		f8_store4<CK>(p, m0 + 16 * (t >> 6) + (t & 15), n, v, f8_bias4<CK>(p, n, flags), flags);
 	}
 }
 
@@ -452,36 +796,130 @@ using namespace s3k;
 
 namespace {
 
-template <int CK>
-int f8_tile_go(F8Args &a, int flags, hipStream_t st)
+template <int CK, int BM, int BN, int WM, int WN, int KS>
+int f8_tile_run(F8Args &a, int flags, hipStream_t st)
 {
-	constexpr int BM = 64, BN = 64;
 	a.nmt = (a.M + BM - 1) / BM, a.nnt = (a.N + BN - 1) / BN;
 	const long long blocks = (long long)a.nmt * a.nnt;
 	if (blocks > 0x7FFFFFFFll)
 		return (int)hipErrorInvalidValue;
-	hipLaunchKernelGGL((f8_tile<CK, BM, BN, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, st, a, flags);
+	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3((unsigned)blocks), dim3(64 * WM * WN * KS), 0, st,
+			   a, flags);
 	return (int)hipGetLastError();
 }
 
-template <int XK, int CK>
-int f8_rows_go(const F8Args &a, int flags, hipStream_t st)
+template <int XK, int CK, int MT>
+int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 {
-	const unsigned blocks = (unsigned)((a.N + 15) / 16);
-	if (a.M <= 16)
-		hipLaunchKernelGGL((f8_rows<XK, CK, 1>), dim3(blocks), dim3(512), 0, st, a, flags);
-	else
-		hipLaunchKernelGGL((f8_rows<XK, CK, 2>), dim3(blocks), dim3(512), 0, st, a, flags);
+	const unsigned mb = (unsigned)((a.M + 16 * MT - 1) / (16 * MT));
+	a.nr = 16;
+	/* a row or a few of x cost little in every workgroup: 4 or 8 weight rows
+	 * each where 16 leave CUs idle (1 x 1024 x 4096: 6.1 us on 64 workgroups) */
+	if (a.M <= 4)
+		while (a.nr > 4 && (a.N + a.nr - 1) / a.nr < 256)
+			a.nr /= 2;
+	const unsigned nb = (unsigned)((a.N + a.nr - 1) / a.nr);
+	/* as many waves as there are blocks of k for, up to 16 (8 with two row
+	 * tiles, for their LDS) */
+	if constexpr (MT == 1) {
+		if (a.KB > 8) {
+			hipLaunchKernelGGL((f8_rows<XK, CK, MT, 16>), dim3(nb, mb), dim3(1024), 0, st, a, flags);
+			return (int)hipGetLastError();
+		}
+	}
+	hipLaunchKernelGGL((f8_rows<XK, CK, MT, 8>), dim3(nb, mb), dim3(512), 0, st, a, flags);
 	return (int)hipGetLastError();
+}
+
+/*
+ * The kernel of a product, by an estimate of each one's time from its grid.
+ * Measured (bf16, 12 row counts from 17 to 20736 by five N x K, and 8192^3),
+ * the tile kernels take, in us, for a block of k with one workgroup on a CU
+ * and with all that fit, and for the rest of a tile; a round is one
+ * workgroup in every place. The few-rows kernels are linear in their
+ * workgroups. Estimate and measurement differ by up to a fifth, near the
+ * borders by less than the choice is worth. Examples, us:
+ *
+ *     M x N x K          64  64/2  64/4   128  192x256  256  rows 1  2
+ *     77 x 1024 x 4096  14.0  10.5   9.7  24.7    40.0  49.4   6.0   4.3
+ *     400 x 1024 x 4096 14.4  10.9  10.1  24.9    41.3  50.4  17.7  13.2
+ *     1369 x 4096 x 1024 14.1 16.8  25.4  12.0    15.4  18.7  79    69
+ *     20736 x 4096 x 1024 163  199   338   118     107   114
+ *     8192^3             850              555     545   470
+ *
+ * (64/2: two groups of waves share out the blocks.) The two largest tiles
+ * are not built for f32 outputs, whose wider operands spill there.
+ */
+enum { F8_T64, F8_T64K2, F8_T64K4, F8_T128, F8_T192, F8_T256, F8_ROWS1, F8_ROWS2, F8_KERNELS };
+
+struct F8Cost {
+	int bm, bn, ks, fit;    /* tile, groups along k, workgroups a CU     */
+	double one, full, rest;
+};
+const F8Cost f8_costs[F8_ROWS1] = {
+	{64, 64, 1, 4, 0.40, 0.83, 1.4},  {64, 64, 2, 2, 0.48, 0.90, 1.8}, {64, 64, 4, 1, 0.87, 0.95, 2.2},
+	{128, 128, 1, 2, 0.75, 1.08, 3.0}, {192, 256, 1, 1, 1.22, 1.42, 3.4}, {256, 256, 1, 1, 1.50, 1.83, 3.7},
+};
+
+double f8_estimate(int kernel, int M, int N, int KB)
+{
+	if (kernel >= F8_ROWS1) {
+		const int mt = kernel == F8_ROWS1 ? 1 : 2;
+		const double wgs = (double)((N + 15) / 16) * ((M + 16 * mt - 1) / (16 * mt));
+		return mt == 1 ? 2.4 + 0.04 * KB + wgs * (0.27e-3 * KB + 0.5e-3)
+			       : 2.7 + 0.05 * KB + wgs * (0.30e-3 * KB + 3.0e-3);
+	}
+	const F8Cost &c = f8_costs[kernel];
+	const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), its = (KB + c.ks - 1) / c.ks;
+	const double places = 256.0 * c.fit, rounds = (double)(long long)(tiles / places);
+	double t = 2.3 + rounds * (its * c.full + c.rest);
+	const double left = tiles - rounds * places;
+	if (left > 0.0) {
+		/* the last round, ceil(left / 256) workgroups on a CU */
+		const double on = (double)(long long)((left + 255.0) / 256.0);
+		const double per = c.fit > 1 ? c.one + (c.full - c.one) * (on - 1.0) / (c.fit - 1.0) : c.one;
+		t += its * per + c.rest;
+	}
+	return t;
+}
+
+template <int CK>
+int f8_product(F8Args &a, int flags, hipStream_t st)
+{
+	int best = F8_T64;
+	double least = 1e30;
+	for (int k = 0; k < F8_KERNELS; ++k) {
+		if ((CK == S3K_F32 && (k == F8_T192 || k == F8_T256)) || (k >= F8_ROWS1 && a.M > 4096))
+			continue;
+		const double t = f8_estimate(k, a.M, a.N, a.KB);
+		if (t < least)
+			least = t, best = k;
+	}
+	switch (best) {
+	case F8_T64K2: return f8_tile_run<CK, 64, 64, 2, 2, 2>(a, flags, st);
+	case F8_T64K4: return f8_tile_run<CK, 64, 64, 2, 2, 4>(a, flags, st);
+	case F8_T128: return f8_tile_run<CK, 128, 128, 2, 2, 1>(a, flags, st);
+	case F8_T192:
+		if constexpr (CK != S3K_F32)
+			return f8_tile_run<CK, 192, 256, 2, 4, 1>(a, flags, st);
+		break;
+	case F8_T256:
+		if constexpr (CK != S3K_F32)
+			return f8_tile_run<CK, 256, 256, 4, 2, 1>(a, flags, st);
+		break;
+	case F8_ROWS1: return f8_rows_go<-1, CK, 1>(a, flags, st);
+	case F8_ROWS2: return f8_rows_go<-1, CK, 2>(a, flags, st);
+	}
+	return f8_tile_run<CK, 64, 64, 2, 2, 1>(a, flags, st);
 }
 
 template <int XK>
-int f8_rows_ck(const F8Args &a, int ck, int flags, hipStream_t st)
+int f8_rows_ck(F8Args &a, int ck, int flags, hipStream_t st)
 {
 	switch (ck) {
-	case S3K_F32: return f8_rows_go<XK, S3K_F32>(a, flags, st);
-	case S3K_F16: return f8_rows_go<XK, S3K_F16>(a, flags, st);
-	case S3K_BF16: return f8_rows_go<XK, S3K_BF16>(a, flags, st);
+	case S3K_F32: return f8_rows_go<XK, S3K_F32, 1>(a, flags, st);
+	case S3K_F16: return f8_rows_go<XK, S3K_F16, 1>(a, flags, st);
+	case S3K_BF16: return f8_rows_go<XK, S3K_BF16, 1>(a, flags, st);
 	}
 	return (int)hipErrorInvalidValue;
 }
@@ -497,6 +935,9 @@ F8Args f8_args(const void *w, const float *sw, void *c, int ck, int M, int N, in
 	a.w = (const uint8_t *)w, a.sw = sw, a.c = c, a.bias = bias;
 	a.M = M, a.N = N, a.K = K, a.KB = (K + F8_BLK - 1) / F8_BLK;
 	a.vec = N % 4 == 0 && (uintptr_t)c % (ck == S3K_F32 ? 16 : 8) == 0;
+	if (N % 8 == 0 && (uintptr_t)c % 16 == 0)
+		a.vec = 2;
+	a.bvec = bias && (uintptr_t)bias % (ck == S3K_F32 ? 16 : 8) == 0;
 	return a;
 }
 
@@ -512,14 +953,10 @@ extern "C" int s3k_fp8_quantize(int kind, const void *x, long long ldx, int rows
 	if (blocks > 0x7FFFFFFFll)
 		return (int)hipErrorInvalidValue;
 	hipStream_t st = (hipStream_t)stream;
-	const bool vec = vec16(x, ldx, kind);
-#define F8_Q(KIND)                                                                                   \
-	if (vec)                                                                                     \
-		hipLaunchKernelGGL((f8_quant_rows<KIND, true>), dim3((unsigned)blocks), dim3(256), 0, st, \
-				   x, ldx, rows, K, KB, (uint8_t *)q, scale);                        \
-	else                                                                                         \
-		hipLaunchKernelGGL((f8_quant_rows<KIND, false>), dim3((unsigned)blocks), dim3(256), 0, \
-				   st, x, ldx, rows, K, KB, (uint8_t *)q, scale)
+	const int vec = vec16(x, ldx, kind);
+#define F8_Q(KIND)                                                                                  \
+	hipLaunchKernelGGL((f8_quant_rows<KIND>), dim3((unsigned)blocks), dim3(256), 0, st, x, ldx, rows, K, \
+			   KB, vec, (uint8_t *)q, scale)
 	switch (kind) {
 	case S3K_F32: F8_Q(S3K_F32); break;
 	case S3K_F16: F8_Q(S3K_F16); break;
@@ -552,11 +989,16 @@ extern "C" int s3k_fp8_matmul(const void *q, const float *sa, const void *w, con
 	F8Args a = f8_args(w, sw, c, ck, M, N, K, bias);
 	a.a = (const uint8_t *)q, a.sa = sa;
 	switch (ck) {
-	case S3K_F32: return f8_tile_go<S3K_F32>(a, flags, (hipStream_t)stream);
-	case S3K_F16: return f8_tile_go<S3K_F16>(a, flags, (hipStream_t)stream);
-	case S3K_BF16: return f8_tile_go<S3K_BF16>(a, flags, (hipStream_t)stream);
+	case S3K_F32: return f8_product<S3K_F32>(a, flags, (hipStream_t)stream);
+	case S3K_F16: return f8_product<S3K_F16>(a, flags, (hipStream_t)stream);
+	case S3K_BF16: return f8_product<S3K_BF16>(a, flags, (hipStream_t)stream);
 	}
 	return (int)hipErrorInvalidValue;
+}
+
+extern "C" int s3k_fp8_rows_ok(int xk, const void *x, long long ldx, int M, int K)
+{
+	return M <= S3K_FP8_ROWS_MAX && K % 8 == 0 && vec16(x, ldx, xk);
 }
 
 extern "C" int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,
@@ -564,10 +1006,10 @@ extern "C" int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w,
 {
 	if (M == 0 || N == 0)
 		return (int)hipSuccess;
-	if (M > S3K_FP8_ROWS_MAX)
+	if (!s3k_fp8_rows_ok(xk, x, ldx, M, K))
 		return (int)hipErrorInvalidValue;
 	F8Args a = f8_args(w, sw, c, ck, M, N, K, bias);
-	a.x = x, a.ldx = ldx, a.xvec = vec16(x, ldx, xk);
+	a.x = x, a.ldx = ldx;
 	switch (xk) {
 	case S3K_F32: return f8_rows_ck<S3K_F32>(a, ck, flags, (hipStream_t)stream);
 	case S3K_F16: return f8_rows_ck<S3K_F16>(a, ck, flags, (hipStream_t)stream);

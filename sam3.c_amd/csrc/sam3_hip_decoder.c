@@ -131,7 +131,7 @@ static size_t fp8_rows_bytes(int M, int K, size_t *total)
 size_t sam3_hip_linear_fp8_work(int M, int N, int K)
 {
 	size_t total;
-	if (M <= S3K_FP8_ROWS_MAX || N <= 0 || K <= 0)
+	if (M <= 0 || N <= 0 || K <= 0)
 		return 0;
 	(void)fp8_rows_bytes(M, K, &total);
 	return total;
@@ -154,26 +154,26 @@ enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, c
 		return SAM3_OK;
 	if (K > 0 && (!x || (uintptr_t)x % esize(x_dtype)))
 		REFUSE(SAM3_EINVAL, "linear_fp8: x is NULL or not element-aligned");
-	if (M <= S3K_FP8_ROWS_MAX)
+	if (s3k_fp8_rows_ok(x_dtype, x, ldx, M, K))
 		return s3h_hip(s3k_fp8_rows(x_dtype, x, ldx, w, w_scale, c_dtype, c, M, N, K, bias, flags,
 					    stream),
 			       "linear_fp8");
-	const size_t need = sam3_hip_linear_fp8_work(M, N, K);
+	size_t need;
+	const size_t scales = fp8_rows_bytes(M, K, &need);
 	void *own = NULL;
 	if (work && (work_bytes < need || (uintptr_t)work % 16))
 		REFUSE(SAM3_EINVAL, "linear_fp8: %zu bytes of work space, %zu needed (16-byte aligned)",
 		       work_bytes, need);
 	if (!work && need) {
 		if (captured(stream))
-			REFUSE(SAM3_EINVAL, "linear_fp8: a captured call of %d rows needs %zu bytes of "
-			       "work space from the caller", M, need);
+			REFUSE(SAM3_EINVAL, "linear_fp8: a captured call of %d rows of %d values needs %zu "
+			       "bytes of work space from the caller", M, K, need);
 		err = s3h_scratch_alloc(&own, need, stream);
 		if (err != SAM3_OK)
 			return err;
 		work = own;
 	}
-	size_t total;
-	float *scale = (float *)((char *)work + fp8_rows_bytes(M, K, &total));
+	float *scale = (float *)((char *)work + scales);
 	err = s3h_hip(s3k_fp8_quantize(x_dtype, x, ldx, M, K, work, scale, stream), "linear_fp8 quantize");
 	if (err == SAM3_OK)
 		err = s3h_hip(s3k_fp8_matmul(work, scale, w, w_scale, c_dtype, c, M, N, K, bias, flags,

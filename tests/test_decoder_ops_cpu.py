@@ -58,7 +58,7 @@ def test_fp8_refusals():
     for work, n in ((OK, need - 1), (OK + 8, need)):
         assert lin(abi.F32, OK, 130, OK, OK, abi.F32, OK, 1000, 4, 130, None, 0, work, n,
                    None) == abi.EINVAL
-    assert hip.linear_fp8_work(1, 4096, 4096) == 0
+    assert hip.linear_fp8_work(1, 4096, 4096) == 4096 + 32 * 4
     assert hip.linear_fp8_work(1000, 0, 128) == 0 and hip.linear_fp8_work(1000, 8, 0) == 0
 
 

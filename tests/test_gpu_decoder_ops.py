@@ -187,7 +187,7 @@ def product64(av, sa, wv, sw, N, K, bias, gelu, c_dt):
     """float64 result and its bound for values av [M, Kp], scales sa [KB, M],
     wv [N, Kp], sw [NB, KB]."""
     M, kb = av.shape[0], av.shape[1] // 128
-    y, mag, cut = (torch.zeros(M, N, dtype=torch.float64) for _ in range(3))
+    y, mag, cut = (torch.zeros(M, N, dtype=torch.float64, device=av.device) for _ in range(3))
     for b in range(kb):
         a, w = av[:, 128 * b:128 * b + 128], wv[:, 128 * b:128 * b + 128]
         s = sa[b][:, None] * sw[:, b].repeat_interleave(128)[:N]
@@ -243,6 +243,33 @@ def test_matmul_fp8(c_dt, M, N, K, flags):
     assert (c[M] == 7.0).all()
 
 
+@pytest.mark.parametrize("c_dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("M,N,K,flags", [
+    (300, 702, 4100, hip.BIAS), (900, 1500, 300, 0), (700, 3001, 200, hip.BIAS), (390, 1001, 4000, 0),
+    (390, 1004, 4000, hip.BIAS | hip.GELU), (400, 900, 2000, 0), (400, 905, 2000, hip.GELU),
+    (1500, 3100, 700, hip.BIAS | hip.GELU), (1500, 3101, 700, 0), (2500, 4000, 260, hip.BIAS | hip.GELU),
+    (2491, 4003, 260, hip.BIAS), (3000, 5000, 1100, hip.BIAS | hip.GELU), (2990, 4999, 1100, 0),
+    (2990, 4996, 1100, hip.BIAS)])
+def test_matmul_fp8_large(c_dt, M, N, K, flags):
+    """Every tile size and both splits of k, with ends inside tiles and rows
+    of whole 16 bytes, 8 and neither. The float64 form runs on the GPU."""
+    g = rng(M + N)
+    kb = -(-K // 128)
+    av = torch.zeros(M, kb * 128)
+    av[:, :K] = torch.randn(M, K, generator=g) * 60.0
+    a8 = av.clamp(-448, 448).to(torch.float8_e4m3fn).cuda()
+    sa = (torch.rand(kb, M, generator=g) * 0.02 + 1e-4).cuda()
+    w8, sw = (t.cuda() for t in weights(g, N, K))
+    bias = torch.randn(N, generator=g).to(TT[c_dt]).cuda()
+    c = torch.full((M + 1, N), 7.0, dtype=TT[c_dt], device="cuda")
+    hip.matmul_fp8_dev(a8.data_ptr(), sa.data_ptr(), w8.data_ptr(), sw.data_ptr(), c_dt, c.data_ptr(), M, N, K,
+                       bias.data_ptr() if flags & hip.BIAS else None, flags, stream())
+    ref, tol = product64(a8.float().double(), sa.double(), w8.float().double(), sw.double(), N, K,
+                         bias.double() if flags & hip.BIAS else None, bool(flags & hip.GELU), c_dt)
+    within(c[:M], ref.cpu(), tol.cpu(), f"{M}x{N}x{K}")
+    assert (c[M] == 7.0).all()
+
+
 def test_matmul_fp8_k0_and_nan():
     c = torch.full((40, 9), 7.0, device="cuda")
     bias = torch.arange(9.0, device="cuda")
@@ -291,6 +318,24 @@ def test_linear_fp8(dt, M, N, K, pad, flags):
     within(c, ref, tol, f"{M}x{N}x{K}")
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("M", [2, 16, 40])
+def test_linear_fp8_nan_and_infinity(dt, M):
+    """An infinity or NaN makes its row NaN and no other."""
+    g = rng(70 + M)
+    N, K = 70, 264
+    x = torch.randn(M, K, generator=g)
+    x[0, 5], x[M - 1, 263] = math.inf, math.nan
+    x = x.to(TT[dt])
+    w8, sw = weights(g, N, K)
+    c = linear(dt, abi.F32, x.cuda(), w8.cuda(), sw.cuda(), N, K, None, 0)
+    assert c[0].isnan().all() and c[M - 1].isnan().all()
+    if M > 2:
+        av, sa, _ = e4m3_groups(x[1:M - 1].double(), 1, K)
+        ref, tol = product64(av, sa.t(), w8.float().double(), sw.double(), N, K, None, False, abi.F32)
+        within(c[1:M - 1], ref, tol, "other rows")
+
+
 def test_linear_fp8_is_quantize_and_matmul():
     """Beyond the fused rows: the same bits as the two calls, from the
     library's scratch as from the caller's work space; x 2 bytes off."""
@@ -330,7 +375,7 @@ def test_linear_fp8_captured(env):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             st = stream()
-            if need:
+            if M > 16:
                 with pytest.raises(hip.HipError):
                     hip.linear_fp8_dev(abi.F32, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32,
                                        c.data_ptr(), M, N, K, stream=st)
