@@ -27,6 +27,7 @@ struct XaArgs {
 	struct s3k_xattn d;
 	int G, rows;            /* query heads per key head; Sq * G          */
 	int nrb, ns;            /* row blocks per (b, h'); parts of the keys */
+	int run;                /* key heads kept on one XCD (xa_place)      */
 	float c;                /* scale * log2(e)                           */
 	int ovec;               /* 4 values of an output row stored together */
 	float *part;            /* ns > 1: results of the parts              */
@@ -42,24 +43,29 @@ __device__ __forceinline__ int xa_len(const int *lens, int b, int most)
 	return n < 0 ? 0 : n > most ? most : n;
 }
 
-/* workgroup -> (b * Hkv + h', part, row block): workgroups go to the 8
- * XCDs round-robin, so the row blocks that read the same keys get ids of
- * one residue mod 8 and share an XCD's L2 */
+/* workgroup -> (b * Hkv + h', part, row block): workgroups go to the 8 XCDs
+ * round-robin. The row blocks that read the same keys get ids of one
+ * residue mod 8 and share an XCD's L2, and so do p.run key heads whose rows
+ * lie together in less than 256 bytes: apart, two XCDs each fetched the
+ * same lines (16 x 8 heads of 16 f32, 5184 keys: 34 us, together 26). */
 __device__ __forceinline__ void xa_place(const XaArgs &p, unsigned id, int &bh, int &part, int &rb)
 {
-	const unsigned combos = (unsigned)(p.d.B * p.d.Hkv * p.ns), nrb = (unsigned)p.nrb;
-	const unsigned whole = combos / 8u * 8u * nrb;
-	unsigned c;
+	const unsigned runs = (unsigned)(p.d.Hkv / p.run), units = (unsigned)(p.d.B * p.ns) * runs;
+	const unsigned per = (unsigned)(p.run * p.nrb), whole = units / 8u * 8u * per;
+	unsigned u, in;
 	if (id < whole) {
 		const unsigned sl = id >> 3;
-		c = sl / nrb * 8u + (id & 7u);
-		rb = (int)(sl % nrb);
+		u = sl / per * 8u + (id & 7u);
+		in = sl % per;
 	} else {
-		c = combos / 8u * 8u + (id - whole) / nrb;
-		rb = (int)((id - whole) % nrb);
+		u = units / 8u * 8u + (id - whole) / per;
+		in = (id - whole) % per;
 	}
-	bh = (int)(c / (unsigned)p.ns);
-	part = (int)(c % (unsigned)p.ns);
+	const unsigned rest = u / runs;
+	const int hk = (int)(u % runs) * p.run + (int)(in / (unsigned)p.nrb);
+	rb = (int)(in % (unsigned)p.nrb);
+	part = (int)(rest % (unsigned)p.ns);
+	bh = (int)(rest / (unsigned)p.ns) * p.d.Hkv + hk;
 }
 
 /* the results of one part: for every (part, b * Hkv + h', row) DP sums,
@@ -83,9 +89,14 @@ __device__ __forceinline__ void xa_out4(const XaArgs &p, long long at, int d, fl
 	}
 	const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-	for (int e = 0; e < 4; ++e)
-		if (d + e < p.d.D)
-			store_from_f32(p.d.out, at + d + e, KIND, x[e]);
+	for (int e = 0; e < 4; ++e) {
+		if (d + e >= p.d.D)
+			return;
+		if constexpr (KIND == S3K_F32)
+			((float *)p.d.out)[at + d + e] = x[e];
+		else
+			((uint16_t *)p.d.out)[at + d + e] = (uint16_t)at_pack2<KIND>(x[e], 0.0f);
+	}
 }
 
 __device__ __forceinline__ long long xa_orow(const XaArgs &p, int bh, int r)
@@ -164,11 +175,12 @@ __global__ void __launch_bounds__(256) xa_generic(XaArgs p)
  * and the probabilities are, as they lie, the P^T operand of
  * O^T = V^T P^T (its k order is permuted alike for both operands).
  * NWQ waves take different rows of the same keys (many rows), NWK waves
- * different key tiles for the same rows (few rows; their results are
- * merged through LDS at the end). K and V tiles of KT keys arrive by
- * direct-to-LDS loads, chunks of 16 bytes XOR-swizzled by the key; one
- * stage is filled while the other is used. Keys past the length and
- * columns past D read as zeros and cost no traffic.
+ * different key tiles for the same rows (few rows; each then loads its own
+ * tiles and meets the others only when their results are merged through
+ * LDS at the end). K and V tiles of KT keys arrive by direct-to-LDS loads,
+ * chunks of 16 bytes XOR-swizzled by the key, in a ring of NST stages.
+ * Keys past the length and columns past D read as zeros and cost no
+ * traffic.
  */
 template <int DP>
 __device__ __forceinline__ int xa_kswz(int key)
@@ -196,20 +208,30 @@ __device__ __forceinline__ int xa_vswz(int key)
  * 2^8, well inside f16, and most tiles pass without a rescale. */
 constexpr float XA_SLACK = 8.0f;
 
-template <int KIND, int DP, int NWQ, int NWK, int KT>
-__global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
+template <int N>
+struct xa_int {
+	static constexpr int value = N;
+};
+
+template <int KIND, int DP, int NWQ, int NWK, int KT, int NST>
+__global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArgs p)
 {
-	constexpr int NW = NWQ * NWK, CH = DP / 8, TB = KT * DP * 2, NMD = DP / 32, NC = DP / 16, NH = KT / 32;
+	/* waves that load a tile together: all, or (one wave of rows) each its own */
+	constexpr bool PRIV = NWQ == 1;
+	constexpr int LW = PRIV ? 1 : NWQ, CH = DP / 8, TB = KT * DP * 2, NMD = DP / 32, NC = DP / 16, NH = KT / 32;
 	constexpr int FAM = KIND == S3K_F16 ? FAM_F16 : FAM_BF16;
-	constexpr int TI = TB / 1024, PER = NWK * TI / NW; /* 1 KiB loads: per tile, per wave */
-	static_assert(NWK * TI % NW == 0, "loads divide over the waves");
-	constexpr int MERGE = (NWK - 1) * NWQ * (NMD * 16 + 2) * 256, STAGE = 2 * NWK * TB;
-	constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
+	constexpr int TI = TB / 1024, PER = TI / LW; /* 1 KiB loads: per tile, per wave */
+	static_assert(NST == 2 || NST == 4, "the ring is unrolled");
+	static_assert(TI % LW == 0 && (PRIV || NWK == 1), "loads divide over the waves");
+	constexpr int MERGE = (NWK - 1) * NWQ * (NMD * 16 + 2) * 256, STAGE = 2 * TB;
+	constexpr int RING = (PRIV ? NWK : 1) * NST * STAGE, LDS = RING > MERGE ? RING : MERGE;
 	__shared__ __attribute__((aligned(1024))) char smem[LDS];
 	const int lane = threadIdx.x & 63, h = lane >> 5, l32 = lane & 31;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int wq = wave % NWQ, wk = wave / NWQ;
-	const unsigned lds0 = lds_addr_of(smem);
+	const int lw = PRIV ? 0 : wave; /* place among the waves that load */
+	char *const ring = smem + (PRIV ? wk * NST * STAGE : 0);
+	const unsigned lds0 = lds_addr_of(ring);
 
 	int bh, part, rb;
 	xa_place(p, blockIdx.x, bh, part, rb);
@@ -244,21 +266,24 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
 	int krow[PER];
 #pragma unroll
 	for (int t = 0; t < PER; ++t) {
-		const int slot = (wave + t * NW) % TI * 64 + lane, row = slot / CH, pos = slot % CH;
+		const int slot = (lw + t * LW) * 64 + lane, row = slot / CH, pos = slot % CH;
 		const int kc = pos ^ xa_kswz<DP>(row), vc = pos ^ xa_vswz<DP>(row);
 		krow[t] = row;
 		koff[t] = 8 * kc < p.d.D ? (unsigned)(row * (int)p.d.k_s + 8 * kc) * 2u : S3K_OOB;
 		voff[t] = 8 * vc < p.d.D ? (unsigned)(row * (int)p.d.v_s + 8 * vc) * 2u : S3K_OOB;
 	}
-	auto issue = [&](int tb, unsigned slot) {
+	/* a tile (past the keys: zeros): every stage is the same number of loads
+	 * to wait for */
+	auto issue = [&](int tile, unsigned slot) {
+		const int key0 = tile * KT;
+		const s3k_i32x4 rk = buf_rsrc(K0 + key0 * p.d.k_s, 0x7FFFFFFFu);
+		const s3k_i32x4 rv = buf_rsrc(V0 + key0 * p.d.v_s, 0x7FFFFFFFu);
 #pragma unroll
 		for (int t = 0; t < PER; ++t) {
-			const int j = wave + t * NW, key0 = (tb + j / TI) * KT;
+			const unsigned at = lds0 + slot + (lw + t * LW) * 1024;
 			const bool in = krow[t] < kn - key0;
-			dma16s(lds0 + slot + j * 1024, buf_rsrc(K0 + key0 * p.d.k_s, 0x7FFFFFFFu),
-			       in ? koff[t] : S3K_OOB, 0);
-			dma16s(lds0 + slot + NWK * TB + j * 1024, buf_rsrc(V0 + key0 * p.d.v_s, 0x7FFFFFFFu),
-			       in ? voff[t] : S3K_OOB, 0);
+			dma16s(at, rk, in ? koff[t] : S3K_OOB, 0);
+			dma16s(at + TB, rv, in ? voff[t] : S3K_OOB, 0);
 		}
 	};
 
@@ -276,21 +301,28 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
 			o[md][e] = 0.0f;
 	float m = XA_NONE, l = 0.0f; /* l: of this half of the lanes' keys */
 
-	const int its = (t1 - t0 + NWK - 1) / NWK;
-	if (its > 0)
-		issue(t0, 0);
-	for (int it = 0; it < its; ++it) {
-		const unsigned slot = (unsigned)(it & 1) * STAGE;
-		wait_vm<0>();
-		__syncthreads();
-		if (it + 1 < its)
-			issue(t0 + (it + 1) * NWK, STAGE - slot);
+	const int its = (t1 - t0 + NWK - 1) / NWK, tw = t0 + (PRIV ? wk : 0);
+#pragma unroll
+	for (int t = 0; t < NST - 1; ++t)
+		issue(tw + t * NWK, t * STAGE);
+	auto step = [&](auto par, int it) __attribute__((always_inline)) {
+		constexpr unsigned slot = decltype(par)::value * STAGE, fill = (decltype(par)::value + NST - 1) % NST * STAGE;
+		/* the tile has landed (everywhere past the barrier), and the stage
+		 * filled now has been read */
+		wait_vm<(NST - 2) * 2 * PER>();
+		if constexpr (PRIV)
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+		else
+			__syncthreads();
+		issue(tw + (it + NST - 1) * NWK, fill);
+		const char *const kt = ring + slot, *const vt = kt + TB;
 		const int tile = t0 + it * NWK + wk;
 		if (!wave_live || tile >= t1)
-			continue;
-		const char *kt = smem + slot + wk * TB, *vt = smem + slot + NWK * TB + wk * TB;
+			return;
 		const int key0 = tile * KT;
 
+		/* its products before another wave's softmax: 1-2 % at D >= 128 */
+		__builtin_amdgcn_s_setprio(1);
 		s3k_f32x16 s[NH];
 #pragma unroll
 		for (int mb = 0; mb < NH; ++mb) {
@@ -303,6 +335,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
 				mfma_chunk<FAM>(s[mb], *(const uint4 *)(kt + row * DP * 2 + (((2 * c + h) ^ xa_kswz<DP>(row)) << 4)),
 						qf[c]);
 		}
+		__builtin_amdgcn_s_setprio(0);
 		if (key0 + KT > kn) {
 #pragma unroll
 			for (int mb = 0; mb < NH; ++mb)
@@ -354,7 +387,19 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
 					mfma_chunk<FAM>(o[md], make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), ph);
 				}
 			}
+	};
+	for (int it = 0; it < its; it += NST) {
+		step(xa_int<0>{}, it);
+		if (it + 1 < its)
+			step(xa_int<1>{}, it + 1);
+		if constexpr (NST == 4) {
+			if (it + 2 < its)
+				step(xa_int<2>{}, it + 2);
+			if (it + 3 < its)
+				step(xa_int<3>{}, it + 3);
+		}
 	}
+	wait_vm<0>(); /* the stages asked for past the part, all zeros */
 	l = at_sum_pair(l);
 
 	if constexpr (NWK > 1) {
@@ -419,8 +464,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
 /* ------------------------------------------------------------------ */
 /*
  * v_mfma_f32_16x16x4_f32 keeps f32 products exact to a rounding. A wave
- * holds RT tiles of 16 rows and takes 16 keys at a time, straight from
- * memory into registers, without LDS: lane (i = lane & 15, g = lane >> 4)
+ * holds RT tiles of 16 rows and takes 16 UN keys at a time, straight from
+ * memory into registers, without LDS, the next ones' loads under way (NB =
+ * 2, where the registers allow): lane (i = lane & 15, g = lane >> 4)
  * reads 16 bytes of key i at d = 16 j + 4 g (k index g of the product with
  * element e is d = 16 j + 4 g + e for both operands), which gives S^T with
  * row i's scores of keys 4 g + 0..3 in its lane; they are the P^T operand
@@ -429,10 +475,16 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_mfma(XaArgs p)
  * u VW + w). Waves of a workgroup take different rows (NWQ) or different
  * keys (NWK), merged through LDS.
  */
+constexpr int xa_f32_un(int dp)
+{
+	return dp == 16 ? 4 : dp == 32 ? 2 : 1;
+}
+
 template <int DP, int RT, int NWQ, int NWK>
-__global__ void __launch_bounds__(64 * NWQ * NWK) xa_f32(XaArgs p)
+__global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 {
 	constexpr int NT = DP / 16, VW = NT < 4 ? NT : 4, NU = NT / VW;
+	constexpr int UN = xa_f32_un(DP), KT = 16 * UN, NB = DP <= 64 ? 2 : 1;
 	constexpr int MV = RT * (NT * 4 + 2); /* values a lane merges */
 	__shared__ float red[NWK > 1 ? (NWK - 1) * NWQ * MV * 64 : 1];
 	const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -458,7 +510,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_f32(XaArgs p)
 				qf[t][j] = *(const float4 *)(Q + 16 * j + 4 * g);
 		}
 	}
-	const int tiles = (kn + 15) / 16;
+	const int tiles = (kn + KT - 1) / KT;
 	const int t0 = (int)((long long)tiles * part / p.ns), t1 = (int)((long long)tiles * (part + 1) / p.ns);
 	const float *K0 = (const float *)p.d.k + b * p.d.k_b + hk * p.d.k_h;
 	const float *V0 = (const float *)p.d.v + b * p.d.v_b + hk * p.d.v_h;
@@ -472,57 +524,72 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_f32(XaArgs p)
 		for (int j = 0; j < NT; ++j)
 			o[t][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 	}
-	for (int tile = t0 + wk; tile < (rw < qn ? t1 : 0); tile += NWK) {
-		const int key0 = tile * 16, left = kn - key0;
-		float4 kf[NT];
-		const float *Kr = K0 + (long long)(key0 + i) * p.d.k_s + 4 * g;
+	float4 kf[NB][UN][NT];
+	float vf[NB][UN][4][NU][VW];
+	auto load = [&](auto buf, int tile) __attribute__((always_inline)) {
+		constexpr int P = decltype(buf)::value;
 #pragma unroll
-		for (int j = 0; j < NT; ++j) {
-			kf[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			if (i < left && 16 * j + 4 * g < D)
-				kf[j] = *(const float4 *)(Kr + 16 * j);
-		}
-		float vf[4][NU][VW];
+		for (int n = 0; n < UN; ++n) {
+			const int key0 = tile * KT + 16 * n, left = kn - key0;
+			const float *Kr = K0 + (long long)(key0 + i) * p.d.k_s + 4 * g;
 #pragma unroll
-		for (int e = 0; e < 4; ++e) {
-			const float *Vr = V0 + (long long)(key0 + 4 * g + e) * p.d.v_s;
+			for (int j = 0; j < NT; ++j) {
+				kf[P][n][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				if (i < left && 16 * j + 4 * g < D)
+					kf[P][n][j] = *(const float4 *)(Kr + 16 * j);
+			}
 #pragma unroll
-			for (int u = 0; u < NU; ++u) {
-				const int d = 16 * VW * u + VW * i;
+			for (int e = 0; e < 4; ++e) {
+				const float *Vr = V0 + (long long)(key0 + 4 * g + e) * p.d.v_s;
 #pragma unroll
-				for (int w = 0; w < VW; ++w)
-					vf[e][u][w] = 0.0f;
-				/* D is a multiple of 4 and d of VW: VW values all count or none do */
-				if (4 * g + e < left && d < D) {
-					if constexpr (VW == 4) {
-						const float4 x = *(const float4 *)(Vr + d);
-						vf[e][u][0] = x.x, vf[e][u][1] = x.y, vf[e][u][2] = x.z, vf[e][u][3] = x.w;
-					} else if constexpr (VW == 2) {
-						const float2 x = *(const float2 *)(Vr + d);
-						vf[e][u][0] = x.x, vf[e][u][1] = x.y;
-					} else {
-						vf[e][u][0] = Vr[d];
+				for (int u = 0; u < NU; ++u) {
+					const int d = 16 * VW * u + VW * i;
+					float (&x)[VW] = vf[P][n][e][u];
+#pragma unroll
+					for (int w = 0; w < VW; ++w)
+						x[w] = 0.0f;
+					/* D is a multiple of 4 and d of VW: all count or none */
+					if (4 * g + e < left && d < D) {
+						if constexpr (VW == 4) {
+							const float4 y = *(const float4 *)(Vr + d);
+							x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+						} else if constexpr (VW == 2) {
+							const float2 y = *(const float2 *)(Vr + d);
+							x[0] = y.x, x[1] = y.y;
+						} else {
+							x[0] = Vr[d];
+						}
 					}
 				}
 			}
 		}
+	};
+	auto work = [&](auto buf, int tile) __attribute__((always_inline)) {
+		constexpr int P = decltype(buf)::value;
+		const int left = kn - tile * KT;
 #pragma unroll
 		for (int t = 0; t < RT; ++t) {
-			s3k_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+			s3k_f32x4 s[UN];
+			float mt = -__builtin_inff();
 #pragma unroll
-			for (int j = 0; j < NT; ++j) {
-				s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].x, qf[t][j].x, s, 0, 0, 0);
-				s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].y, qf[t][j].y, s, 0, 0, 0);
-				s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].z, qf[t][j].z, s, 0, 0, 0);
-				s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j].w, qf[t][j].w, s, 0, 0, 0);
-			}
-			if (left < 16) {
+			for (int n = 0; n < UN; ++n) {
+				s[n] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-				for (int e = 0; e < 4; ++e)
-					if (4 * g + e >= left)
-						s[e] = -__builtin_inff();
+				for (int j = 0; j < NT; ++j) {
+					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].x, qf[t][j].x, s[n], 0, 0, 0);
+					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].y, qf[t][j].y, s[n], 0, 0, 0);
+					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].z, qf[t][j].z, s[n], 0, 0, 0);
+					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].w, qf[t][j].w, s[n], 0, 0, 0);
+				}
+				if (left < KT) {
+#pragma unroll
+					for (int e = 0; e < 4; ++e)
+						if (16 * n + 4 * g + e >= left)
+							s[n][e] = -__builtin_inff();
+				}
+				mt = fmaxf(mt, fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
 			}
-			float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * p.c;
+			mt *= p.c;
 			mt = fmaxf(mt, __shfl_xor(mt, 16));
 			mt = at_max_pair(mt);
 			if (__any(mt > m[t] + XA_SLACK)) {
@@ -536,16 +603,41 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_f32(XaArgs p)
 						o[t][j][e] *= al;
 			}
 #pragma unroll
-			for (int e = 0; e < 4; ++e) {
-				const float pe = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -m[t]));
-				l[t] += pe;
+			for (int n = 0; n < UN; ++n)
 #pragma unroll
-				for (int u = 0; u < NU; ++u)
+				for (int e = 0; e < 4; ++e) {
+					const float pe = __builtin_amdgcn_exp2f(fmaf(s[n][e], p.c, -m[t]));
+					l[t] += pe;
 #pragma unroll
-					for (int w = 0; w < VW; ++w)
-						o[t][u * VW + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][u][w], pe,
-													o[t][u * VW + w], 0, 0, 0);
-			}
+					for (int u = 0; u < NU; ++u)
+#pragma unroll
+						for (int w = 0; w < VW; ++w)
+							o[t][u * VW + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+								vf[P][n][e][u][w], pe, o[t][u * VW + w], 0, 0, 0);
+				}
+		}
+	};
+	xa_int<0> b0;
+	xa_int<NB - 1> b1;
+	const int end = rw < qn ? t1 : 0;
+	int tile = t0 + wk;
+	if constexpr (NB == 1) {
+		for (; tile < end; tile += NWK) {
+			load(b0, tile);
+			work(b0, tile);
+		}
+	} else {
+		if (tile < end)
+			load(b0, tile);
+		for (; tile < end; tile += 2 * NWK) {
+			if (tile + NWK < end)
+				load(b1, tile + NWK);
+			work(b0, tile);
+			if (tile + NWK >= end)
+				break;
+			if (tile + 2 * NWK < end)
+				load(b0, tile + 2 * NWK);
+			work(b1, tile + NWK);
 		}
 	}
 #pragma unroll
@@ -619,9 +711,10 @@ __global__ void __launch_bounds__(64 * NWQ * NWK) xa_f32(XaArgs p)
 	}
 }
 
-/* The parts of a row joined: DP / 4 lanes take a row, four values each. */
+/* The parts of a row joined, many rows: DP / 4 lanes take a row, four
+ * values each, part by part. */
 template <int KIND, int DP>
-__global__ void __launch_bounds__(256) xa_join(XaArgs p)
+__global__ void __launch_bounds__(256) xa_join_many(XaArgs p)
 {
 	constexpr int L = DP / 4;
 	const long long rows = (long long)(p.d.B * p.d.Hkv) * p.rows, row = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -636,6 +729,7 @@ __global__ void __launch_bounds__(256) xa_join(XaArgs p)
 		m = fmaxf(m, pm[s * rows + row]);
 	float l = 0.0f;
 	float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
 	for (int s = 0; s < p.ns; ++s) {
 		const float a = __builtin_amdgcn_exp2f(pm[s * rows + row] - m);
 		const float4 v = *(const float4 *)(p.part + (s * rows + row) * DP + d);
@@ -644,6 +738,64 @@ __global__ void __launch_bounds__(256) xa_join(XaArgs p)
 	}
 	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 	xa_out4<KIND>(p, xa_orow(p, bh, r), d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+/*
+ * The parts of a row joined, few rows: a workgroup per row, DP / 4 lanes with
+ * four values each times NG groups, which share out the parts (one after the
+ * other, 78 parts of a 40000-key row took 35 us of loads) and are added up
+ * in LDS in order.
+ */
+template <int KIND, int DP>
+__global__ void __launch_bounds__(256) xa_join(XaArgs p)
+{
+	constexpr int L = DP / 4, NG = 256 / L;
+	__shared__ float4 so[NG][L];
+	__shared__ float sm[4], sl[NG];
+	const long long rows = (long long)(p.d.B * p.d.Hkv) * p.rows, row = blockIdx.x;
+	const int bh = (int)(row / p.rows), r = (int)(row - (long long)bh * p.rows);
+	if (r >= xa_len(p.d.q_len, bh / p.d.Hkv, p.d.Sq) * p.G)
+		return;
+	const float *pm = p.part + rows * p.ns * DP, *pl = pm + rows * p.ns;
+	const int li = threadIdx.x % L, grp = threadIdx.x / L;
+	/* this thread's first parts are asked for before the maximum is known */
+	const bool have = grp < p.ns;
+	float4 v = have ? *(const float4 *)(p.part + (grp * rows + row) * DP + 4 * li) : make_float4(0, 0, 0, 0);
+	float vm = have ? pm[grp * rows + row] : XA_NONE, vl = have ? pl[grp * rows + row] : 0.0f;
+	float m = XA_NONE;
+	for (int s = threadIdx.x; s < p.ns; s += 256)
+		m = fmaxf(m, pm[s * rows + row]);
+	m = wave_max_f32(m);
+	if ((threadIdx.x & 63) == 0)
+		sm[threadIdx.x >> 6] = m;
+	__syncthreads();
+	m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+	float l = 0.0f;
+	float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+	for (int s = grp; s < p.ns; s += NG) {
+		const float a = __builtin_amdgcn_exp2f(vm - m);
+		l = fmaf(vl, a, l);
+		o.x = fmaf(v.x, a, o.x), o.y = fmaf(v.y, a, o.y), o.z = fmaf(v.z, a, o.z), o.w = fmaf(v.w, a, o.w);
+		if (s + NG < p.ns) {
+			const long long at = (s + NG) * rows + row;
+			v = *(const float4 *)(p.part + at * DP + 4 * li);
+			vm = pm[at], vl = pl[at];
+		}
+	}
+	so[grp][li] = o;
+	if (li == 0)
+		sl[grp] = l;
+	__syncthreads();
+	if (grp > 0)
+		return;
+	const int n = p.ns < NG ? p.ns : NG;
+	for (int g = 1; g < n; ++g) {
+		const float4 u = so[g][li];
+		o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
+		l += sl[g];
+	}
+	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+	xa_out4<KIND>(p, xa_orow(p, bh, r), 4 * li, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 } /* namespace s3k */
@@ -664,12 +816,12 @@ bool xa_16(const void *p, long long strides, int es)
 
 /* Waves along the rows and along the keys, and keys per step. */
 struct XaShape {
-	int dp, rows, nwk, kt;
+	int dp, rows, nwk, kt, fit; /* fit: workgroups a CU */
 };
 
 XaShape xa_shape(const struct s3k_xattn *d, int path)
 {
-	XaShape s = {xa_dp(d->D), 0, 1, 16};
+	XaShape s = {xa_dp(d->D), 0, 1, 16, 2};
 	const long long rows = (long long)d->Sq * (d->H / d->Hkv);
 	if (path == S3K_XATTN_MFMA) {
 		if (s.dp < 32)
@@ -677,11 +829,13 @@ XaShape xa_shape(const struct s3k_xattn *d, int path)
 		const bool few = rows <= 32;
 		s.rows = few ? 32 : 128;
 		s.nwk = few ? (s.dp == 256 ? 2 : 4) : 1;
-		s.kt = s.dp == 256 || (few && s.dp == 128) ? 32 : 64;
+		s.kt = few || s.dp == 256 ? 32 : 64;
+		s.fit = few && s.dp >= 128 ? 1 : 2;
 	} else if (path == S3K_XATTN_F32) {
 		const bool few = rows <= 16;
-		s.rows = few ? 16 : 64;
+		s.rows = few ? 16 : s.dp == 256 ? 64 : 128;
 		s.nwk = few ? 4 : 1;
+		s.kt = 16 * xa_f32_un(s.dp);
 	}
 	return s;
 }
@@ -690,11 +844,11 @@ template <int KIND, int DP>
 int xa_go16(const XaArgs &a, const XaShape &s, unsigned blocks, hipStream_t st)
 {
 	if (s.rows == 32) {
-		constexpr int NWK = DP == 256 ? 2 : 4, KT = DP >= 128 ? 32 : 64;
-		hipLaunchKernelGGL((xa_mfma<KIND, DP, 1, NWK, KT>), dim3(blocks), dim3(64 * NWK), 0, st, a);
+		constexpr int NWK = DP == 256 ? 2 : 4, NST = DP == 32 ? 4 : 2;
+		hipLaunchKernelGGL((xa_mfma<KIND, DP, 1, NWK, 32, NST>), dim3(blocks), dim3(64 * NWK), 0, st, a);
 	} else {
 		constexpr int KT = DP == 256 ? 32 : 64;
-		hipLaunchKernelGGL((xa_mfma<KIND, DP, 4, 1, KT>), dim3(blocks), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_mfma<KIND, DP, 4, 1, KT, 2>), dim3(blocks), dim3(256), 0, st, a);
 	}
 	return (int)hipGetLastError();
 }
@@ -716,23 +870,33 @@ int xa_gof(const XaArgs &a, const XaShape &s, unsigned blocks, hipStream_t st)
 	if (s.rows == 16)
 		hipLaunchKernelGGL((xa_f32<DP, 1, 1, 4>), dim3(blocks), dim3(256), 0, st, a);
 	else
-		hipLaunchKernelGGL((xa_f32<DP, 1, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_f32<DP, DP == 256 ? 1 : 2, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
+	return (int)hipGetLastError();
+}
+
+template <int KIND, int DP>
+int xa_joined(const XaArgs &a, hipStream_t st)
+{
+	const long long rows = (long long)a.d.B * a.d.Hkv * a.rows, per = 256 / (DP / 4);
+	/* 5184 rows of 12 parts: 15 us by lanes, 35 by workgroups; 16 rows of 78
+	 * parts 38 and 5 */
+	if (rows > 1024)
+		hipLaunchKernelGGL((xa_join_many<KIND, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a);
+	else
+		hipLaunchKernelGGL((xa_join<KIND, DP>), dim3((unsigned)rows), dim3(256), 0, st, a);
 	return (int)hipGetLastError();
 }
 
 template <int KIND>
 int xa_joined(const XaArgs &a, int dp, hipStream_t st)
 {
-	const long long rows = (long long)a.d.B * a.d.Hkv * a.rows, per = 256 / (dp / 4);
-	const unsigned blocks = (unsigned)((rows + per - 1) / per);
 	switch (dp) {
-	case 16: hipLaunchKernelGGL((xa_join<KIND, 16>), dim3(blocks), dim3(256), 0, st, a); break;
-	case 32: hipLaunchKernelGGL((xa_join<KIND, 32>), dim3(blocks), dim3(256), 0, st, a); break;
-	case 64: hipLaunchKernelGGL((xa_join<KIND, 64>), dim3(blocks), dim3(256), 0, st, a); break;
-	case 128: hipLaunchKernelGGL((xa_join<KIND, 128>), dim3(blocks), dim3(256), 0, st, a); break;
-	default: hipLaunchKernelGGL((xa_join<KIND, 256>), dim3(blocks), dim3(256), 0, st, a); break;
+	case 16: return xa_joined<KIND, 16>(a, st);
+	case 32: return xa_joined<KIND, 32>(a, st);
+	case 64: return xa_joined<KIND, 64>(a, st);
+	case 128: return xa_joined<KIND, 128>(a, st);
+	default: return xa_joined<KIND, 256>(a, st);
 	}
-	return (int)hipGetLastError();
 }
 
 } /* namespace */
@@ -767,11 +931,18 @@ extern "C" int s3k_xattn_parts(const struct s3k_xattn *d, int path)
 	const XaShape s = xa_shape(d, path);
 	const long long rows = (long long)d->Sq * (d->H / d->Hkv);
 	const long long wgs = (rows + s.rows - 1) / s.rows * d->B * d->Hkv;
-	/* two workgroups per CU, each with at least four steps */
-	long long parts = 512 / (wgs ? wgs : 1);
-	const long long most = d->Sk / (4ll * s.kt * s.nwk);
+	/* the places for workgroups filled once. Many rows: each with at least
+	 * four steps (400 rows x 1000 keys 14.9 us, with one 18.4); few rows: with
+	 * one (2000 keys 8.5 us, with four 10.2), from four on (500 keys 6.9 us
+	 * in one part, 8.0 in two), and no more parts than a join reads quickly
+	 * (40000 keys 16.4 us in 78, 19.3 in 128) */
+	const long long step = (long long)s.kt * s.nwk, few = s.nwk > 1;
+	long long parts = 256 * s.fit / (wgs ? wgs : 1);
+	const long long most = few ? (d->Sk >= 4 * step ? d->Sk / step : 1) : d->Sk / (4 * step);
 	if (parts > most)
 		parts = most;
+	if (parts > 64)
+		parts = 64;
 	return parts < 2 ? 1 : (int)parts;
 }
 
@@ -816,6 +987,10 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 	if (blocks > 0x7FFFFFFFll)
 		return (int)hipErrorInvalidValue;
 	a.nrb = (int)nrb;
+	const int es = d->kind == S3K_F32 ? 4 : 2;
+	a.run = 1;
+	while (d->Hkv % (2 * a.run) == 0 && 2 * a.run * d->k_h * es <= 256)
+		a.run *= 2;
 	int rc;
 	if (path == S3K_XATTN_MFMA) {
 		rc = d->kind == S3K_F16 ? xa_go16<S3K_F16>(a, s, (unsigned)blocks, st)
