@@ -414,7 +414,8 @@ enum sam3_error sam3_hip_sdpa_on_path(int path, int dtype, const void *q, const 
 /* each row and block, stored block-major [KB, rows]; weights one for   */
 /* each 128 x 128 block, [ceil(N / 128), KB]. Quantized tensors are     */
 /* 16-byte aligned, scales 4-byte aligned. Outputs must not overlap     */
-/* inputs.                                                              */
+/* inputs. As for every call here, the device of the pointers and of    */
+/* the stream has to be the calling thread's current one.               */
 /* ------------------------------------------------------------------ */
 
 /* x [rows, K] (F32, F16 or BF16, rows ldx elements apart, ldx >= K) -> q
@@ -438,7 +439,8 @@ enum sam3_error sam3_hip_fp8_quantize_weight(int w_dtype, const void *w, long lo
  * a[m,k] * w[n,k]). a_scale and w_scale are any f32 values (not only
  * powers of two). Sums, bias and GELU are f32, then one rounding to
  * c_dtype (F32, F16 or BF16); bias [N] is of c_dtype. Rows of C are dense.
- * flags: SAM3_HIP_BIAS | SAM3_HIP_GELU. K = 0 gives zeros (and the bias).
+ * flags: SAM3_HIP_BIAS | SAM3_HIP_GELU, others are SAM3_EINVAL. K = 0 gives
+ * zeros (and the bias); K is at most 2^22.
  * For F16 and BF16 outputs the products of each group of 8 consecutive k
  * are added on a grid of 2^-13 of the group's largest, what lies below cut
  * off (the 8-bit matrix instruction's arithmetic: about 1.4e-5 of a result
@@ -450,8 +452,9 @@ enum sam3_error sam3_hip_matmul_fp8(const void *a, const float *a_scale, const v
 
 /* The whole layer: x [M, K] (F32, F16 or BF16, rows ldx elements apart)
  * quantized as sam3_hip_fp8_quantize does, then sam3_hip_matmul_fp8. Up to
- * 16 rows, 16-byte aligned and of a multiple of 8 values, are quantized
- * inside the product's kernel: the same quantized values, sums in another
+ * 16 rows, 16-byte aligned and of a multiple of 8 values, may be quantized
+ * inside the product's kernel (where that is quicker, or the call is
+ * captured without work space): the same quantized values, sums in another
  * order. Other calls need sam3_hip_linear_fp8_work(M, N, K) bytes for the
  * quantized copy: `work` (16-byte aligned, at least that many bytes, not
  * used by anything else until the call's work is done) or, with work NULL,
@@ -519,7 +522,8 @@ enum sam3_error sam3_hip_norm_rope(const struct sam3_hip_norm_rope *p, void *str
  *     `slow` times are divided by factor, with a ramp linear in the turns
  *     between; *amp = 0.1 ln(factor) + 1.
  * *amp is 1 for the first two. SAM3_EINVAL: rot odd or negative, theta <= 0,
- * factor < 1, trained < 1, fast <= slow, or a NULL output. */
+ * factor < 1, trained < 1, slow < 0, fast <= slow, one of them not finite,
+ * or a NULL output. */
 #define SAM3_HIP_ROPE_PLAIN  0
 #define SAM3_HIP_ROPE_LINEAR 1
 #define SAM3_HIP_ROPE_PARTS  2
@@ -538,10 +542,10 @@ enum sam3_error sam3_hip_rope_frequencies(int rot, double theta, int scaling, do
  * a tensor lies at b*x_b + s*x_s + h*x_h + d (strides in elements, >= 0;
  * outputs must not overlap anything). Keys and values at k_len[b] and past
  * are not read, query rows at q_len[b] and past neither read nor written
- * (lengths are clamped to 0..Sk and 0..Sq). A row without keys, or whose
+ * (lengths are clamped to 0..Sk and 0..Sq, Sk is below 2^30). A row without keys, or whose
  * scores are all -inf, gets zeros. Statistics and sums are f32; f16 and
- * bf16 probabilities are rounded to the tensors' type for the product with
- * v, and their sum is that of the rounded values. */
+ * bf16 probabilities may be rounded to the tensors' type for the product
+ * with v, and their sum is then that of the rounded values. */
 struct sam3_hip_cross_attention {
 	int dtype;            /* F32, F16 or BF16, of all four tensors        */
 	int B, H, Hkv;        /* H a multiple of Hkv                          */

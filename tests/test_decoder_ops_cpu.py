@@ -121,6 +121,8 @@ def test_rope_frequencies():
                 (8, 1e4, 3, 1, 1, 2, 1, at, C.byref(a)), (8, 1e4, 1, 0.5, 1, 2, 1, at, C.byref(a)),
                 (8, 1e4, 1, math.inf, 1, 2, 1, at, C.byref(a)),
                 (8, 1e4, 2, 4, 0.5, 2, 1, at, C.byref(a)), (8, 1e4, 2, 4, 10, 1, 1, at, C.byref(a)),
+                (8, 1e4, 2, 4, 10, 4, -math.inf, at, C.byref(a)), (8, 1e4, 2, 4, 10, math.inf, 1, at, C.byref(a)),
+                (8, math.inf, 0, 1, 1, 2, 1, at, C.byref(a)),
                 (8, 1e4, 0, 1, 1, 2, 1, None, C.byref(a)), (8, 1e4, 0, 1, 1, 2, 1, at, None)):
         assert fn(*bad) == abi.EINVAL, bad
 
@@ -149,7 +151,7 @@ def test_cross_attention_refusals():
                 dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=OK + 1), dict(k=OK + 1),
                 dict(v=OK + 1), dict(out=OK + 1), dict(q_len=OK + 2), dict(k_len=OK + 1), dict(q_b=-8),
                 dict(k_s=-8), dict(v_h=-8), dict(o_b=-8), dict(o_s=0), dict(o_h=0), dict(o_b=0),
-                dict(Sq=1 << 30), dict(path=4), dict(path=2),
+                dict(Sq=1 << 30), dict(Sk=1 << 30), dict(path=4), dict(path=2),
                 dict(path=1, D=60), dict(path=1, k=OK + 2), dict(path=1, q_s=12)):
         assert run(**bad) == abi.EINVAL, bad
     need = hip.cross_attention_work(cross())

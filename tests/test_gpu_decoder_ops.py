@@ -319,8 +319,9 @@ def test_linear_fp8(dt, M, N, K, pad, flags):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
-@pytest.mark.parametrize("M", [2, 16, 40])
-def test_linear_fp8_nan_and_infinity(dt, M):
+@pytest.mark.parametrize("c_dt", [abi.F32, abi.BF16], ids=["to-f32", "to-bf16"])
+@pytest.mark.parametrize("M", [2, 16, 40, 700])
+def test_linear_fp8_nan_and_infinity(dt, c_dt, M):
     """An infinity or NaN makes its row NaN and no other."""
     g = rng(70 + M)
     N, K = 70, 264
@@ -328,11 +329,11 @@ def test_linear_fp8_nan_and_infinity(dt, M):
     x[0, 5], x[M - 1, 263] = math.inf, math.nan
     x = x.to(TT[dt])
     w8, sw = weights(g, N, K)
-    c = linear(dt, abi.F32, x.cuda(), w8.cuda(), sw.cuda(), N, K, None, 0)
+    c = linear(dt, c_dt, x.cuda(), w8.cuda(), sw.cuda(), N, K, None, 0)
     assert c[0].isnan().all() and c[M - 1].isnan().all()
     if M > 2:
         av, sa, _ = e4m3_groups(x[1:M - 1].double(), 1, K)
-        ref, tol = product64(av, sa.t(), w8.float().double(), sw.double(), N, K, None, False, abi.F32)
+        ref, tol = product64(av, sa.t(), w8.float().double(), sw.double(), N, K, None, False, c_dt)
         within(c[1:M - 1], ref, tol, "other rows")
 
 
@@ -363,9 +364,8 @@ def test_linear_fp8_captured(env):
     replayed; without it a call that needs some is refused."""
     env.set("SAM3_HIP_QUIET", "1")
     g = rng(4)
-    N, K = 300, 520
-    w8, sw = (t.cuda() for t in weights(g, N, K))
-    for M in (3, 90):
+    for M, N, K in ((3, 300, 520), (90, 300, 520), (16, 100, 4104), (5, 100, 515)):
+        w8, sw = (t.cuda() for t in weights(g, N, K))
         xs = [torch.randn(M, K, generator=g).cuda() for _ in range(3)]
         x, c = xs[0].clone(), torch.empty(M, N, device="cuda")
         need = hip.linear_fp8_work(M, N, K)
@@ -375,17 +375,23 @@ def test_linear_fp8_captured(env):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             st = stream()
-            if M > 16:
+            if M > 16 or K % 8:
                 with pytest.raises(hip.HipError):
                     hip.linear_fp8_dev(abi.F32, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32,
                                        c.data_ptr(), M, N, K, stream=st)
             hip.linear_fp8_dev(abi.F32, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32, c.data_ptr(), M,
                                N, K, work=work.data_ptr(), work_bytes=need, stream=st)
+            if M == 16:  # few rows need no space, if it comes to that
+                c2 = torch.empty_like(c)
+                hip.linear_fp8_dev(abi.F32, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32, c2.data_ptr(), M,
+                                   N, K, stream=st)
         for t, e in zip(xs, eager):
             x.copy_(t)
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(c, e)
+            if M == 16:
+                assert torch.allclose(c2, c, rtol=1e-4, atol=1e-4 * float(c.abs().max()))
             linear(abi.F32, abi.F32, t, w8, sw, N, K, None, 0)  # eager work between the replays
 
 
