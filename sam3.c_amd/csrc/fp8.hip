@@ -550,15 +550,15 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 		const int row = (j < WI ? j : j - WI) * 8 + (lane >> 3);
 		off[t] = (unsigned)row * Kp + (unsigned)(((lane & 7) ^ f8_swz(row)) * 16);
 	}
-	auto issue = [&](int kb, unsigned slot) {
+	auto issue = [&](int t, int kb, unsigned slot) __attribute__((always_inline)) {
 		const bool in = kb < p.KB;
-#pragma unroll
-		for (int t = 0; t < PER; ++t) {
+		if (t < PER) {
 			const int j = wave + t * NW;
 			dma16s(lds0 + slot + j * 1024, j < WI ? rw : ra, in ? off[t] : S3K_OOB, in ? (unsigned)kb * F8_BLK : 0u);
+		} else {
+			const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, in ? (unsigned)arows * 4 : 0u);
+			dma4s(lds0 + slot + WB + AB + wave * 256, rs, (unsigned)(wave * 256 + lane * 4));
 		}
-		const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, in ? (unsigned)arows * 4 : 0u);
-		dma4s(lds0 + slot + WB + AB + wave * 256, rs, (unsigned)(wave * 256 + lane * 4));
 	};
 
 	s3k_f32x4 acc[NT][MT];
@@ -576,7 +576,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 	const float *swp = p.sw + (long long)((n0 + wn * (BN / WN)) / F8_BLK) * p.KB;
 	const bool live = n0 + wn * (BN / WN) < p.N;
 
-	issue(ks, 0);
+#pragma unroll
+	for (int t = 0; t <= PER; ++t)
+		issue(t, ks, 0);
 	unsigned slot = 0;
 	for (int k0 = 0; k0 < p.KB; k0 += KS) {
 		const int kb = k0 + ks;
@@ -584,7 +586,6 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 		 * wave is past the block before, whose stage is filled again */
 		wait_vm<0>();
 		wg_barrier();
-		issue(kb + KS, STAGE - slot);
 		const float sw = live && kb < p.KB ? swp[kb] : 0.0f;
 		const unsigned wat = wo + slot, aat = ao + slot;
 		f8_i8 fa[MT];
@@ -605,6 +606,11 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 		};
 #pragma unroll
 		for (int i = 0; i < NT; ++i) {
+			/* the next block's loads a few at a time: asked for at once they
+			 * kept the waves waiting at the address unit */
+#pragma unroll
+			for (int t = i * (PER + 1) / NT; t < (i + 1) * (PER + 1) / NT; ++t)
+				issue(t, kb + KS, STAGE - slot);
 			const f8_i8 fw = f8_join(lds_rd16(wat + o0, i * 16 * F8_BLK), lds_rd16(wat + o1, i * 16 * F8_BLK));
 #pragma unroll
 			for (int j = 0; j < MT; ++j)

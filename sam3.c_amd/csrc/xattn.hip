@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 	constexpr int LW = PRIV ? 1 : NWQ, CH = DP / 8, TB = KT * DP * 2, NMD = DP / 32, NC = DP / 16, NH = KT / 32;
 	constexpr int FAM = KIND == S3K_F16 ? FAM_F16 : FAM_BF16;
 	constexpr int TI = TB / 1024, PER = TI / LW; /* 1 KiB loads: per tile, per wave */
+	static_assert(64 % CH == 0, "a load is whole rows");
 	static_assert(NST == 2 || NST == 4, "the ring is unrolled");
 	static_assert(TI % LW == 0 && (PRIV || NWK == 1), "loads divide over the waves");
 	constexpr int MERGE = (NWK - 1) * NWQ * (NMD * 16 + 2) * 256, STAGE = 2 * TB;
@@ -262,15 +263,17 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 	const int t0 = (int)((long long)tiles * part / p.ns), t1 = (int)((long long)tiles * (part + 1) / p.ns);
 	const uint16_t *K0 = (const uint16_t *)p.d.k + b * p.d.k_b + hk * p.d.k_h;
 	const uint16_t *V0 = (const uint16_t *)p.d.v + b * p.d.v_b + hk * p.d.v_h;
+	/* load t: key row r0 + t RS of the tile, chunk (lane % CH) ^ swizzle.
+	 * The row's distance from r0 is a scalar offset, so that loads whose
+	 * swizzles agree share one lane offset. */
+	constexpr int RS = LW * 64 / CH;
+	const int r0 = (lw * 64 + lane) / CH, pos = lane % CH;
 	unsigned koff[PER], voff[PER];
-	int krow[PER];
 #pragma unroll
 	for (int t = 0; t < PER; ++t) {
-		const int slot = (lw + t * LW) * 64 + lane, row = slot / CH, pos = slot % CH;
-		const int kc = pos ^ xa_kswz<DP>(row), vc = pos ^ xa_vswz<DP>(row);
-		krow[t] = row;
-		koff[t] = 8 * kc < p.d.D ? (unsigned)(row * (int)p.d.k_s + 8 * kc) * 2u : S3K_OOB;
-		voff[t] = 8 * vc < p.d.D ? (unsigned)(row * (int)p.d.v_s + 8 * vc) * 2u : S3K_OOB;
+		const int kc = pos ^ xa_kswz<DP>(r0 + t * RS), vc = pos ^ xa_vswz<DP>(r0 + t * RS);
+		koff[t] = 8 * kc < p.d.D ? (unsigned)(r0 * (int)p.d.k_s + 8 * kc) * 2u : S3K_OOB;
+		voff[t] = 8 * vc < p.d.D ? (unsigned)(r0 * (int)p.d.v_s + 8 * vc) * 2u : S3K_OOB;
 	}
 	/* a tile (past the keys: zeros): every stage is the same number of loads
 	 * to wait for */
@@ -281,9 +284,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 #pragma unroll
 		for (int t = 0; t < PER; ++t) {
 			const unsigned at = lds0 + slot + (lw + t * LW) * 1024;
-			const bool in = krow[t] < kn - key0;
-			dma16s(at, rk, in ? koff[t] : S3K_OOB, 0);
-			dma16s(at + TB, rv, in ? voff[t] : S3K_OOB, 0);
+			const bool in = r0 < kn - key0 - t * RS;
+			dma16s(at, rk, in ? koff[t] : S3K_OOB, (unsigned)(t * RS * (int)p.d.k_s) * 2u);
+			dma16s(at + TB, rv, in ? voff[t] : S3K_OOB, (unsigned)(t * RS * (int)p.d.v_s) * 2u);
 		}
 	};
 
@@ -321,8 +324,6 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 			return;
 		const int key0 = tile * KT;
 
-		/* its products before another wave's softmax: 1-2 % at D >= 128 */
-		__builtin_amdgcn_s_setprio(1);
 		s3k_f32x16 s[NH];
 #pragma unroll
 		for (int mb = 0; mb < NH; ++mb) {
@@ -335,7 +336,6 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 				mfma_chunk<FAM>(s[mb], *(const uint4 *)(kt + row * DP * 2 + (((2 * c + h) ^ xa_kswz<DP>(row)) << 4)),
 						qf[c]);
 		}
-		__builtin_amdgcn_s_setprio(0);
 		if (key0 + KT > kn) {
 #pragma unroll
 			for (int mb = 0; mb < NH; ++mb)
