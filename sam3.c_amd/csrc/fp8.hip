@@ -511,7 +511,9 @@ __device__ __forceinline__ void f8_place(const F8Args &p, unsigned id, int &mt, 
  * BN/WN in 16x16 MFMA tiles of a whole block of 128 k. A stage holds one
  * block of both operands (rows of 8 16-byte chunks, swizzled) and the
  * rows' scales; two stages in a ring, filled by direct-to-LDS loads a
- * block ahead. KS such groups of waves, each with stages of its own, take
+ * block ahead, over the end of a tile into the next one where a workgroup
+ * takes several (20736 x 4096 x 1024 with GELU: 112 us, a workgroup for
+ * each tile 117). KS such groups of waves, each with stages of its own, take
  * every KS-th block and are added up in LDS: for few tiles, whose blocks
  * one after the other would leave most CUs idle.
  */
@@ -531,13 +533,17 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 	char *const smem = smem_all + ks * NST * STAGE;
 	const unsigned lds0 = lds_addr_of(smem);
 
+	/* the tile whose blocks are asked for */
+	const unsigned Kp = (unsigned)p.KB * F8_BLK, total = (unsigned)p.nmt * (unsigned)p.nnt;
 	int n0, m0;
-	f8_place(p, blockIdx.x, m0, n0);
-	m0 *= BM, n0 *= BN;
-	const unsigned Kp = (unsigned)p.KB * F8_BLK;
-	const int wrows = min(BN, p.N - n0), arows = min(BM, p.M - m0);
-	const s3k_i32x4 rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)wrows * Kp);
-	const s3k_i32x4 ra = buf_rsrc(p.a + (long long)m0 * Kp, (unsigned)arows * Kp);
+	s3k_i32x4 rw, ra;
+	auto place = [&](unsigned id) {
+		f8_place(p, id, m0, n0);
+		m0 *= BM, n0 *= BN;
+		rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)min(BN, p.N - n0) * Kp);
+		ra = buf_rsrc(p.a + (long long)m0 * Kp, (unsigned)min(BM, p.M - m0) * Kp);
+	};
+	place(blockIdx.x);
 
 	/* load j = wave + t * NW: rows 8 j .. 8 j + 7 of W, then of A; rows
 	 * past the end lie past the buffer and read as zeros, and so are
@@ -556,99 +562,110 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 			const int j = wave + t * NW;
 			dma16s(lds0 + slot + j * 1024, j < WI ? rw : ra, in ? off[t] : S3K_OOB, in ? (unsigned)kb * F8_BLK : 0u);
 		} else {
-			const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, in ? (unsigned)arows * 4 : 0u);
+			const s3k_i32x4 rs = buf_rsrc(p.sa + (long long)kb * p.M + m0, in ? (unsigned)min(BM, p.M - m0) * 4 : 0u);
 			dma4s(lds0 + slot + WB + AB + wave * 256, rs, (unsigned)(wave * 256 + lane * 4));
 		}
 	};
-
-	s3k_f32x4 acc[NT][MT];
-#pragma unroll
-	for (int i = 0; i < NT; ++i)
-#pragma unroll
-		for (int j = 0; j < MT; ++j)
-			acc[i][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
 	/* operand row l16 of tile t: chunks g and g + 4 (the swizzle of rows 16
 	 * apart is the same) */
 	const unsigned o0 = (unsigned)(l16 * F8_BLK + ((g ^ f8_swz(l16)) << 4));
 	const unsigned o1 = (unsigned)(l16 * F8_BLK + (((g + 4) ^ f8_swz(l16)) << 4));
 	const unsigned wo = lds0 + wn * (BN / WN) * F8_BLK, ao = lds0 + WB + wm * (BM / WM) * F8_BLK;
-	const float *swp = p.sw + (long long)((n0 + wn * (BN / WN)) / F8_BLK) * p.KB;
-	const bool live = n0 + wn * (BN / WN) < p.N;
-
 #pragma unroll
 	for (int t = 0; t <= PER; ++t)
 		issue(t, ks, 0);
 	unsigned slot = 0;
-	for (int k0 = 0; k0 < p.KB; k0 += KS) {
-		const int kb = k0 + ks;
-		/* block kb has landed here, and everywhere past the barrier; every
-		 * wave is past the block before, whose stage is filled again */
-		wait_vm<0>();
-		wg_barrier();
-		const float sw = live && kb < p.KB ? swp[kb] : 0.0f;
-		const unsigned wat = wo + slot, aat = ao + slot;
-		f8_i8 fa[MT];
-		float s[MT];
+	wait_vm<0>();
+	for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+		/* where this tile lies; m0 and n0 move on to the next one at its end */
+		const int tm = m0, tn = n0 + wn * (BN / WN);
+		const float *swp = p.sw + (long long)(tn / F8_BLK) * p.KB;
+		s3k_f32x4 acc[NT][MT];
 #pragma unroll
-		for (int j = 0; j < MT; ++j) {
-			fa[j] = f8_join(lds_rd16(aat + o0, j * 16 * F8_BLK), lds_rd16(aat + o1, j * 16 * F8_BLK));
-			s[j] = *(const float *)(smem + slot + WB + AB + (wm * (BM / WM) + 16 * j + l16) * 4) * sw;
-		}
-		/* the results of tile row i are added while row i + 1 is formed */
-		s3k_f32x4 z[2][MT];
-		auto add = [&](int i) {
+		for (int i = 0; i < NT; ++i)
 #pragma unroll
 			for (int j = 0; j < MT; ++j)
+				acc[i][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+		for (int k0 = 0; k0 < p.KB; k0 += KS) {
+			const int kb = k0 + ks;
+			int ask = kb + KS;
+			if (k0 + KS >= p.KB && tile + gridDim.x < total) {
+				/* the next tile's first block, before this one's is stored */
+				place(tile + gridDim.x);
+				ask = ks;
+			}
+			/* block kb has landed here, and everywhere past the barrier; every
+			 * wave is past the block before, whose stage is filled again */
+			if (k0 > 0)
+				wait_vm<0>();
+			wg_barrier();
+			const float sw = tn < p.N && kb < p.KB ? swp[kb] : 0.0f;
+			const unsigned wat = wo + slot, aat = ao + slot;
+			f8_i8 fa[MT];
+			float s[MT];
 #pragma unroll
-				for (int r = 0; r < 4; ++r)
-					acc[i][j][r] = fmaf(z[i & 1][j][r], s[j], acc[i][j][r]);
-		};
-#pragma unroll
-		for (int i = 0; i < NT; ++i) {
-			/* the next block's loads a few at a time: asked for at once they
-			 * kept the waves waiting at the address unit */
-#pragma unroll
-			for (int t = i * (PER + 1) / NT; t < (i + 1) * (PER + 1) / NT; ++t)
-				issue(t, kb + KS, STAGE - slot);
-			const f8_i8 fw = f8_join(lds_rd16(wat + o0, i * 16 * F8_BLK), lds_rd16(wat + o1, i * 16 * F8_BLK));
-#pragma unroll
-			for (int j = 0; j < MT; ++j)
-				z[i & 1][j] = f8_mfma16<CK == S3K_F32>(fw, fa[j], (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f});
-			if (i > 0)
-				add(i - 1);
-		}
-		add(NT - 1);
-		slot = STAGE - slot;
-	}
-	wait_vm<0>(); /* the last stage asked for, all zeros */
-	if constexpr (KS > 1) {
-		wg_barrier();
-		float *const sum = (float *)smem_all + wave * (NT * MT * 256) + lane * 4;
-		if (ks > 0) {
-			float *const mine = sum + (ks - 1) * (BM * BN);
-#pragma unroll
-			for (int i = 0; i < NT; ++i)
+			for (int j = 0; j < MT; ++j) {
+				fa[j] = f8_join(lds_rd16(aat + o0, j * 16 * F8_BLK), lds_rd16(aat + o1, j * 16 * F8_BLK));
+				s[j] = *(const float *)(smem + slot + WB + AB + (wm * (BM / WM) + 16 * j + l16) * 4) * sw;
+			}
+			/* the results of tile row i are added while row i + 1 is formed */
+			s3k_f32x4 z[2][MT];
+			auto add = [&](int i) {
 #pragma unroll
 				for (int j = 0; j < MT; ++j)
-					*(s3k_f32x4 *)(mine + (i * MT + j) * 256) = acc[i][j];
-		}
-		__syncthreads();
-		if (ks > 0)
-			return;
-#pragma unroll
-		for (int o = 0; o < KS - 1; ++o)
-#pragma unroll
-			for (int i = 0; i < NT; ++i)
-#pragma unroll
-				for (int j = 0; j < MT; ++j) {
-					const s3k_f32x4 v = *(const s3k_f32x4 *)(sum + o * (BM * BN) + (i * MT + j) * 256);
 #pragma unroll
 					for (int r = 0; r < 4; ++r)
-						acc[i][j][r] += v[r];
-				}
+						acc[i][j][r] = fmaf(z[i & 1][j][r], s[j], acc[i][j][r]);
+			};
+#pragma unroll
+			for (int i = 0; i < NT; ++i) {
+				/* the next block's loads a few at a time: asked for at once they
+				 * kept the waves waiting at the address unit */
+#pragma unroll
+				for (int t = i * (PER + 1) / NT; t < (i + 1) * (PER + 1) / NT; ++t)
+					issue(t, ask, STAGE - slot);
+				const f8_i8 fw = f8_join(lds_rd16(wat + o0, i * 16 * F8_BLK), lds_rd16(wat + o1, i * 16 * F8_BLK));
+#pragma unroll
+				for (int j = 0; j < MT; ++j)
+					z[i & 1][j] = f8_mfma16<CK == S3K_F32>(fw, fa[j], (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f});
+				if (i > 0)
+					add(i - 1);
+			}
+			add(NT - 1);
+			slot = STAGE - slot;
+		}
+		/* the next tile's first block, or zeros: before the stores, which a
+		 * wait after them would wait for too */
+		wait_vm<0>();
+		if constexpr (KS > 1) {
+			wg_barrier();
+			float *const sum = (float *)smem_all + wave * (NT * MT * 256) + lane * 4;
+			if (ks > 0) {
+				float *const mine = sum + (ks - 1) * (BM * BN);
+#pragma unroll
+				for (int i = 0; i < NT; ++i)
+#pragma unroll
+					for (int j = 0; j < MT; ++j)
+						*(s3k_f32x4 *)(mine + (i * MT + j) * 256) = acc[i][j];
+			}
+			__syncthreads();
+			if (ks > 0)
+				return;
+#pragma unroll
+			for (int o = 0; o < KS - 1; ++o)
+#pragma unroll
+				for (int i = 0; i < NT; ++i)
+#pragma unroll
+					for (int j = 0; j < MT; ++j) {
+						const s3k_f32x4 v = *(const s3k_f32x4 *)(sum + o * (BM * BN) + (i * MT + j) * 256);
+#pragma unroll
+						for (int r = 0; r < 4; ++r)
+							acc[i][j][r] += v[r];
+					}
+		}
+		f8_tile_store<CK, NT, MT>(p, acc, tm + wm * (BM / WM) + l16, tn, g, flags);
 	}
-	f8_tile_store<CK, NT, MT>(p, acc, m0 + wm * (BM / WM) + l16, n0 + wn * (BN / WN), g, flags);
 }
 
 /*
@@ -809,8 +826,11 @@ int f8_tile_run(F8Args &a, int flags, hipStream_t st)
 	const long long blocks = (long long)a.nmt * a.nnt;
 	if (blocks > 0x7FFFFFFFll)
 		return (int)hipErrorInvalidValue;
-	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3((unsigned)blocks), dim3(64 * WM * WN * KS), 0, st,
-			   a, flags);
+	/* one workgroup a CU for the tiles that leave room for no more; the
+	 * others overlap their ends by themselves. 256 is a multiple of the XCDs:
+	 * a workgroup's tiles stay on its XCD's run. */
+	const unsigned grid = WM * WN > 4 && a.KB > 0 && blocks > 256 ? 256 : (unsigned)blocks;
+	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3(grid), dim3(64 * WM * WN * KS), 0, st, a, flags);
 	return (int)hipGetLastError();
 }
 
