@@ -358,7 +358,6 @@ struct F8Args {
 	int vec;                /* columns of C stored together: 1 four, 2 also
 				 * eight of 16 bits                          */
 	int bvec;               /* four values of the bias loaded together   */
-	int nr;                 /* f8_rows: weight rows of a workgroup       */
 	/* fused quantization: x in place of a, sa */
 	const void *x;
 	long long ldx;
@@ -669,7 +668,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 }
 
 /*
- * Few rows: a workgroup takes 16 (p.nr) weight rows and 16 MT rows of A;
+ * Few rows: a workgroup takes 16 weight rows and 16 MT rows of A (with 4
+ * weight rows, for more workgroups, 1 x 1024 x 4096 took 3.9 us, with 16 3.5);
  * its NWV waves share out the blocks of k (wave w takes w, w + NWV, ...)
  * and add up in LDS. Every wave has two blocks under way in LDS of its own
  * and meets the others only at the end. The operands come by direct-to-LDS
@@ -696,9 +696,9 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 	float (*const red)[MT][256] = (float (*)[MT][256])smem;
 	const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const int n0 = (int)blockIdx.x * p.nr, m0 = (int)blockIdx.y * 16 * MT;
+	const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * MT;
 	const unsigned Kp = (unsigned)p.KB * F8_BLK;
-	const s3k_i32x4 rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)min(p.nr, p.N - n0) * Kp);
+	const s3k_i32x4 rw = buf_rsrc(p.w + (long long)n0 * Kp, (unsigned)min(16, p.N - n0) * Kp);
 	const s3k_i32x4 ra = buf_rsrc(XK < 0 ? p.a + (long long)m0 * Kp : nullptr,
 				      XK < 0 ? (unsigned)min(16 * MT, p.M - m0) * Kp : 0u);
 	const float *swp = p.sw + (long long)(n0 / F8_BLK) * p.KB;
@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 	__syncthreads();
 	/* thread t < 64 MT: lane t % 64 of tile t / 64, its four columns */
 	const int t = threadIdx.x;
-	if (t < 64 * MT && 4 * ((t & 63) >> 4) < p.nr) {
+	if (t < 64 * MT) {
 		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
 		for (int w = 0; w < NWV; ++w) {
@@ -822,29 +822,25 @@ namespace {
 template <int CK, int BM, int BN, int WM, int WN, int KS>
 int f8_tile_run(F8Args &a, int flags, hipStream_t st)
 {
-	a.nmt = (a.M + BM - 1) / BM, a.nnt = (a.N + BN - 1) / BN;
+	a.nmt = (int)((a.M + BM - 1ll) / BM), a.nnt = (int)((a.N + BN - 1ll) / BN);
 	const long long blocks = (long long)a.nmt * a.nnt;
-	if (blocks > 0x7FFFFFFFll)
-		return (int)hipErrorInvalidValue;
 	/* one workgroup a CU for the tiles that leave room for no more; the
 	 * others overlap their ends by themselves. 256 is a multiple of the XCDs:
 	 * a workgroup's tiles stay on its XCD's run. */
-	const unsigned grid = WM * WN > 4 && a.KB > 0 && blocks > 256 ? 256 : (unsigned)blocks;
-	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3(grid), dim3(64 * WM * WN * KS), 0, st, a, flags);
+	const long long grid = WM * WN > 4 && a.KB > 0 && blocks > 256 ? 256 : blocks;
+	if (blocks > 0x7FFFFFFFll || !s3k_launchable(grid, 64 * WM * WN * KS))
+		return (int)hipErrorInvalidValue;
+	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3((unsigned)grid), dim3(64 * WM * WN * KS), 0, st, a, flags);
 	return (int)hipGetLastError();
 }
 
 template <int XK, int CK, int MT>
 int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 {
-	const unsigned mb = (unsigned)((a.M + 16 * MT - 1) / (16 * MT));
-	a.nr = 16;
-	/* a row or a few of x cost little in every workgroup: 4 or 8 weight rows
-	 * each where 16 leave CUs idle (1 x 1024 x 4096: 6.1 us on 64 workgroups) */
-	if (a.M <= 4)
-		while (a.nr > 4 && (a.N + a.nr - 1) / a.nr < 256)
-			a.nr /= 2;
-	const unsigned nb = (unsigned)((a.N + a.nr - 1) / a.nr);
+	const unsigned mb = (unsigned)((a.M + 16 * MT - 1) / (16 * MT)); /* M is small */
+	const unsigned nb = (unsigned)((a.N + 15ll) / 16);
+	if (!s3k_launchable(nb, 1024))
+		return (int)hipErrorInvalidValue;
 	/* as many waves as there are blocks of k for, up to 16 (8 with two row
 	 * tiles, for their LDS) */
 	if constexpr (MT == 1) {
@@ -859,19 +855,19 @@ int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 
 /*
  * The kernel of a product, by an estimate of each one's time from its grid.
- * Measured (bf16, 12 row counts from 17 to 20736 by five N x K, and 8192^3),
+ * Measured (bf16, 10 row counts from 24 to 20736 by five N x K, and 8192^3),
  * the tile kernels take, in us, for a block of k with one workgroup on a CU
  * and with all that fit, and for the rest of a tile; a round is one
  * workgroup in every place. The few-rows kernels are linear in their
- * workgroups. Estimate and measurement differ by up to a fifth, near the
- * borders by less than the choice is worth. Examples, us:
+ * workgroups. The kernel it takes was at most 12 % behind the quickest, 1 %
+ * in the mean. Examples, us:
  *
- *     M x N x K          64  64/2  64/4   128  192x256  256  rows 1  2
- *     77 x 1024 x 4096  14.0  10.5   9.7  24.7    40.0  49.4   6.0   4.3
- *     400 x 1024 x 4096 14.4  10.9  10.1  24.9    41.3  50.4  17.7  13.2
- *     1369 x 4096 x 1024 14.1 16.8  25.4  12.0    15.4  18.7  79    69
- *     20736 x 4096 x 1024 163  199   338   118     107   114
- *     8192^3             850              555     545   470
+ *     M x N x K            64  64/2  64/4   128  192x256  256  rows 1  2
+ *     77 x 1024 x 4096   16.5  12.1  10.4  25.4    40.2  48.1   5.9   4.2
+ *     400 x 1024 x 4096  16.9  12.4  10.8  26.0    41.4  49.0  17.6  13.0
+ *     1369 x 4096 x 1024 14.5  18.2  27.0  12.3    15.5  17.9  65    71
+ *     20736 x 4096 x 1024 165   209   363   121     106   115  931  1030
+ *     8192^3              850               555     545   470
  *
  * (64/2: two groups of waves share out the blocks.) The two largest tiles
  * are not built for f32 outputs, whose wider operands spill there.
@@ -883,20 +879,20 @@ struct F8Cost {
 	double one, full, rest;
 };
 const F8Cost f8_costs[F8_ROWS1] = {
-	{64, 64, 1, 4, 0.40, 0.83, 1.4},  {64, 64, 2, 2, 0.48, 0.90, 1.8}, {64, 64, 4, 1, 0.87, 0.95, 2.2},
-	{128, 128, 1, 2, 0.75, 1.08, 3.0}, {192, 256, 1, 1, 1.22, 1.42, 3.4}, {256, 256, 1, 1, 1.50, 1.83, 3.7},
+	{64, 64, 1, 4, 0.35, 0.82, 1.0},   {64, 64, 2, 2, 0.61, 0.97, 1.2},   {64, 64, 4, 1, 0.95, 0.95, 1.8},
+	{128, 128, 1, 2, 0.87, 1.22, 1.9}, {192, 256, 1, 1, 1.63, 1.63, 3.9}, {256, 256, 1, 1, 1.60, 1.60, 8.4},
 };
 
 double f8_estimate(int kernel, int M, int N, int KB)
 {
 	if (kernel >= F8_ROWS1) {
 		const int mt = kernel == F8_ROWS1 ? 1 : 2;
-		const double wgs = (double)((N + 15) / 16) * ((M + 16 * mt - 1) / (16 * mt));
-		return mt == 1 ? 2.4 + 0.04 * KB + wgs * (0.27e-3 * KB + 0.5e-3)
-			       : 2.7 + 0.05 * KB + wgs * (0.30e-3 * KB + 3.0e-3);
+		const double wgs = (double)((N + 15ll) / 16) * ((M + 16ll * mt - 1) / (16 * mt));
+		return mt == 1 ? 2.4 + 0.012 * KB + wgs * (0.27e-3 * KB + 0.45e-3)
+			       : 2.3 + 0.029 * KB + wgs * (0.30e-3 * KB + 2.8e-3);
 	}
 	const F8Cost &c = f8_costs[kernel];
-	const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), its = (KB + c.ks - 1) / c.ks;
+	const double tiles = (double)((M + c.bm - 1ll) / c.bm) * ((N + c.bn - 1ll) / c.bn), its = (KB + c.ks - 1) / c.ks;
 	const double places = 256.0 * c.fit, rounds = (double)(long long)(tiles / places);
 	double t = 2.3 + rounds * (its * c.full + c.rest);
 	const double left = tiles - rounds * places;
@@ -976,7 +972,7 @@ extern "C" int s3k_fp8_quantize(int kind, const void *x, long long ldx, int rows
 	const long long blocks = ((long long)rows * KB + 15) / 16;
 	if (blocks == 0)
 		return (int)hipSuccess;
-	if (blocks > 0x7FFFFFFFll)
+	if (!s3k_launchable(blocks, 256))
 		return (int)hipErrorInvalidValue;
 	hipStream_t st = (hipStream_t)stream;
 	const int vec = vec16(x, ldx, kind);
@@ -996,11 +992,11 @@ extern "C" int s3k_fp8_quantize(int kind, const void *x, long long ldx, int rows
 extern "C" int s3k_fp8_quantize_weight(int kind, const void *w, long long ldw, int N, int K, void *q,
 				       float *scale, void *stream)
 {
-	const int KB = (K + F8_BLK - 1) / F8_BLK, NB = (N + F8_BLK - 1) / F8_BLK;
+	const int KB = (K + F8_BLK - 1) / F8_BLK, NB = (int)((N + F8_BLK - 1ll) / F8_BLK);
 	const long long blocks = (long long)KB * NB;
 	if (blocks == 0)
 		return (int)hipSuccess;
-	if (blocks > 0x7FFFFFFFll)
+	if (!s3k_launchable(blocks, 256))
 		return (int)hipErrorInvalidValue;
 	hipLaunchKernelGGL(f8_quant_blocks, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, w,
 			   kind, ldw, N, K, KB, (uint8_t *)q, scale);

@@ -426,6 +426,13 @@ const struct s3h_settings *s3h_settings(void);
  * *bytes is its size. Returns a hipError_t value. */
 int s3k_noalloc_scratch(void **ptr, size_t *bytes);
 
+/* Whether a launch of blocks x threads is within the 2^32 - 1 work-items of
+ * one grid axis. */
+static inline int s3k_launchable(long long blocks, int threads)
+{
+	return blocks >= 0 && blocks <= 0xFFFFFFFFll / threads;
+}
+
 /* ------------------------------------------------------------------ */
 /* e4m3 linear layers (fp8.hip): rows of ceil(K / 128) whole blocks of   */
 /* 128 bytes, scales of rows [KB, rows], of weights [ceil(N / 128), KB]  */
