@@ -415,7 +415,8 @@ enum sam3_error sam3_hip_sdpa_on_path(int path, int dtype, const void *q, const 
 /* each 128 x 128 block, [ceil(N / 128), KB]. Quantized tensors are     */
 /* 16-byte aligned, scales 4-byte aligned. Outputs must not overlap     */
 /* inputs. As for every call here, the device of the pointers and of    */
-/* the stream has to be the calling thread's current one.               */
+/* the stream has to be the calling thread's current one; and problems  */
+/* of more than 2^32 - 1 work-items in a launch are SAM3_EINVAL.         */
 /* ------------------------------------------------------------------ */
 
 /* x [rows, K] (F32, F16 or BF16, rows ldx elements apart, ldx >= K) -> q
@@ -440,7 +441,8 @@ enum sam3_error sam3_hip_fp8_quantize_weight(int w_dtype, const void *w, long lo
  * powers of two). Sums, bias and GELU are f32, then one rounding to
  * c_dtype (F32, F16 or BF16); bias [N] is of c_dtype. Rows of C are dense.
  * flags: SAM3_HIP_BIAS | SAM3_HIP_GELU, others are SAM3_EINVAL. K = 0 gives
- * zeros (and the bias); K is at most 2^22.
+ * zeros (and the bias); K is at most 2^22, M and N at most 2^30. The two
+ * scales are multiplied first: their product has to be finite.
  * For F16 and BF16 outputs the products of each group of 8 consecutive k
  * are added on a grid of 2^-13 of the group's largest, what lies below cut
  * off (the 8-bit matrix instruction's arithmetic: about 1.4e-5 of a result

@@ -306,7 +306,7 @@ extern "C" int s3k_norm_rope(const struct s3k_norm_rope *d, void *stream)
 		a.rc = a.rows;
 	a.nrc = (a.rows + a.rc - 1) / a.rc;
 	const long long blocks = (a.T + a.tpb - 1) / a.tpb * a.nrc;
-	if (blocks > 0x7FFFFFFFll)
+	if (!s3k_launchable(blocks, 256))
 		return (int)hipErrorInvalidValue;
 	hipStream_t st = (hipStream_t)stream;
 	switch (d->kind) {

@@ -44,13 +44,23 @@ static int captured(void *stream)
 /* e4m3 linear layers                                                   */
 /* ------------------------------------------------------------------ */
 #define FP8_MAX_K (1 << 22) /* 256 rows of a tile stay below 2^31 bytes */
+#define FP8_MAX_ROWS (1 << 30) /* of either operand: a tile's last row is an int */
+
+/* The result of a launcher: one that finds more workgroups than a launch
+ * takes returns hipErrorInvalidValue before any. */
+static enum sam3_error launched(int e, const char *what)
+{
+	if (e == hipErrorInvalidValue)
+		REFUSE(SAM3_EINVAL, "%s: more workgroups than one launch takes", what);
+	return s3h_hip(e, what);
+}
 
 static enum sam3_error fp8_quant_check(const char *what, int dtype, const void *x, long long ld,
 				       int rows, int K, const void *q, const void *scale)
 {
 	if (!is_float_dtype(dtype))
 		REFUSE(SAM3_EDTYPE, "%s: dtype %d is not F32, F16 or BF16", what, dtype);
-	if (rows < 0 || K < 0 || K > FP8_MAX_K || ld < K)
+	if (rows < 0 || rows > FP8_MAX_ROWS || K < 0 || K > FP8_MAX_K || ld < K)
 		REFUSE(SAM3_EINVAL, "%s: rows=%d K=%d ld=%lld", what, rows, K, ld);
 	if (rows == 0 || K == 0)
 		return SAM3_OK;
@@ -68,7 +78,7 @@ enum sam3_error sam3_hip_fp8_quantize(int x_dtype, const void *x, long long ldx,
 	const enum sam3_error err = fp8_quant_check("fp8_quantize", x_dtype, x, ldx, rows, K, q, scale);
 	if (err != SAM3_OK)
 		return err;
-	return s3h_hip(s3k_fp8_quantize(x_dtype, x, ldx, rows, K, q, scale, stream), "fp8_quantize");
+	return launched(s3k_fp8_quantize(x_dtype, x, ldx, rows, K, q, scale, stream), "fp8_quantize");
 }
 
 enum sam3_error sam3_hip_fp8_quantize_weight(int w_dtype, const void *w, long long ldw, int N, int K,
@@ -78,7 +88,7 @@ enum sam3_error sam3_hip_fp8_quantize_weight(int w_dtype, const void *w, long lo
 		fp8_quant_check("fp8_quantize_weight", w_dtype, w, ldw, N, K, q, scale);
 	if (err != SAM3_OK)
 		return err;
-	return s3h_hip(s3k_fp8_quantize_weight(w_dtype, w, ldw, N, K, q, scale, stream),
+	return launched(s3k_fp8_quantize_weight(w_dtype, w, ldw, N, K, q, scale, stream),
 		       "fp8_quantize_weight");
 }
 
@@ -89,7 +99,7 @@ static enum sam3_error fp8_product_check(const char *what, const void *w, const 
 {
 	if (!is_float_dtype(c_dtype))
 		REFUSE(SAM3_EDTYPE, "%s: output dtype %d is not F32, F16 or BF16", what, c_dtype);
-	if (M < 0 || N < 0 || K < 0 || K > FP8_MAX_K)
+	if (M < 0 || M > FP8_MAX_ROWS || N < 0 || N > FP8_MAX_ROWS || K < 0 || K > FP8_MAX_K)
 		REFUSE(SAM3_EINVAL, "%s: M=%d N=%d K=%d", what, M, N, K);
 	if (flags & ~(SAM3_HIP_BIAS | SAM3_HIP_GELU))
 		REFUSE(SAM3_EINVAL, "%s: unknown flags %d", what, flags);
@@ -116,7 +126,7 @@ enum sam3_error sam3_hip_matmul_fp8(const void *a, const float *a_scale, const v
 		REFUSE(SAM3_EINVAL, "matmul_fp8: NULL pointer");
 	if ((uintptr_t)a % 16 || (uintptr_t)a_scale % 4)
 		REFUSE(SAM3_EINVAL, "matmul_fp8: a must be 16-byte, a_scale 4-byte aligned");
-	return s3h_hip(s3k_fp8_matmul(a, a_scale, w, w_scale, c_dtype, c, M, N, K, bias, flags, stream),
+	return launched(s3k_fp8_matmul(a, a_scale, w, w_scale, c_dtype, c, M, N, K, bias, flags, stream),
 		       "matmul_fp8");
 }
 
@@ -159,7 +169,7 @@ enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, c
 	 * 8 x 4096 x 4096 6.4 and 6.3; 16 x 1024 x 1024 5.2 and 3.6). */
 	if (s3k_fp8_rows_ok(x_dtype, x, ldx, M, K) &&
 	    ((long long)M * ((K + 127) / 128) <= 256 || (!work && captured(stream))))
-		return s3h_hip(s3k_fp8_rows(x_dtype, x, ldx, w, w_scale, c_dtype, c, M, N, K, bias, flags,
+		return launched(s3k_fp8_rows(x_dtype, x, ldx, w, w_scale, c_dtype, c, M, N, K, bias, flags,
 					    stream),
 			       "linear_fp8");
 	size_t need;
@@ -178,9 +188,9 @@ enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, c
 		work = own;
 	}
 	float *scale = (float *)((char *)work + scales);
-	err = s3h_hip(s3k_fp8_quantize(x_dtype, x, ldx, M, K, work, scale, stream), "linear_fp8 quantize");
+	err = launched(s3k_fp8_quantize(x_dtype, x, ldx, M, K, work, scale, stream), "linear_fp8 quantize");
 	if (err == SAM3_OK)
-		err = s3h_hip(s3k_fp8_matmul(work, scale, w, w_scale, c_dtype, c, M, N, K, bias, flags,
+		err = launched(s3k_fp8_matmul(work, scale, w, w_scale, c_dtype, c, M, N, K, bias, flags,
 					     stream),
 			      "linear_fp8");
 	const enum sam3_error ferr = s3h_scratch_free(own, stream);
@@ -255,7 +265,7 @@ enum sam3_error sam3_hip_norm_rope(const struct sam3_hip_norm_rope *p, void *str
 					p->layout == SAM3_HIP_ROPE_HALF, heads_of(&p->q),
 					heads_of(&p->k), p->pos, p->pos_b, p->freq, p->amp,
 					p->norm != 0, p->eps};
-	return s3h_hip(s3k_norm_rope(&d, stream), "norm_rope");
+	return launched(s3k_norm_rope(&d, stream), "norm_rope");
 }
 
 enum sam3_error sam3_hip_rope_frequencies(int rot, double theta, int scaling, double factor,
@@ -374,7 +384,7 @@ enum sam3_error sam3_hip_cross_attention_on_path(int path, const struct sam3_hip
 		}
 		work = own;
 	}
-	err = s3h_hip(s3k_xattn_run(&d, path, parts, work, stream), "cross_attention");
+	err = launched(s3k_xattn_run(&d, path, parts, work, stream), "cross_attention");
 	const enum sam3_error ferr = s3h_scratch_free(own, stream);
 	return err != SAM3_OK ? err : ferr;
 }

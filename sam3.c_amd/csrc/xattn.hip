@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) xa_generic(XaArgs p)
 		}
 	}
 	/* no key, or no score above -inf: zeros (a NaN sum stays one) */
-	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+	const float inv = 1.0f / l;
 	const long long at = xa_orow(p, bh, r);
 #pragma unroll
 	for (int i = 0; i < 4; ++i)
@@ -448,15 +448,17 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArg
 		}
 		return;
 	}
-	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+	/* no key, or no score above -inf: zeros, also where 0 * v is NaN */
+	const bool none = l == 0.0f;
+	const float inv = 1.0f / l;
 	const long long at = xa_orow(p, bh, r);
 #pragma unroll
 	for (int md = 0; md < NMD; ++md)
 #pragma unroll
 		for (int g = 0; g < 4; ++g)
 			xa_out4<KIND>(p, at, 32 * md + 8 * g + 4 * h,
-				      make_float4(o[md][4 * g] * inv, o[md][4 * g + 1] * inv,
-						  o[md][4 * g + 2] * inv, o[md][4 * g + 3] * inv));
+				      make_float4(none ? 0.0f : o[md][4 * g] * inv, none ? 0.0f : o[md][4 * g + 1] * inv,
+						  none ? 0.0f : o[md][4 * g + 2] * inv, none ? 0.0f : o[md][4 * g + 3] * inv));
 }
 
 /* ------------------------------------------------------------------ */
@@ -684,7 +686,8 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 		const int r = rw + 16 * t + i;
 		if (r >= qn)
 			continue;
-		const float inv = p.ns > 1 ? 1.0f : l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+		const bool none = p.ns == 1 && l[t] == 0.0f;
+		const float inv = p.ns > 1 ? 1.0f : 1.0f / l[t];
 		const long long pr = xa_prow(p, part, bh, r), all = (long long)p.ns * (p.d.B * p.d.Hkv) * p.rows;
 		const long long at = xa_orow(p, bh, r);
 		/* tile u VW + w, register e: d = 16 VW u + VW (4 g + e) + w. As
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 				float v[4];
 #pragma unroll
 				for (int x = 0; x < 4; ++x)
-					v[x] = o[t][u * VW + x % VW][n * (4 / VW) + x / VW] * inv;
+					v[x] = none ? 0.0f : o[t][u * VW + x % VW][n * (4 / VW) + x / VW] * inv;
 				const int d = 16 * VW * u + VW * 4 * g + 4 * n;
 				const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
 				if (p.ns > 1)
@@ -709,6 +712,14 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 			p.part[all * (DP + 1) + pr] = l[t];
 		}
 	}
+}
+
+/* o / l; a row of no key, or no score above -inf: zeros, also where o is NaN
+ * (0 times an infinite v) */
+__device__ __forceinline__ float4 xa_over(const float4 &o, float l)
+{
+	const float inv = 1.0f / l;
+	return l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 /* The parts of a row joined, many rows: DP / 4 lanes take a row, four
@@ -736,8 +747,7 @@ __global__ void __launch_bounds__(256) xa_join_many(XaArgs p)
 		l = fmaf(pl[s * rows + row], a, l);
 		o.x = fmaf(v.x, a, o.x), o.y = fmaf(v.y, a, o.y), o.z = fmaf(v.z, a, o.z), o.w = fmaf(v.w, a, o.w);
 	}
-	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-	xa_out4<KIND>(p, xa_orow(p, bh, r), d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+	xa_out4<KIND>(p, xa_orow(p, bh, r), d, xa_over(o, l));
 }
 
 /*
@@ -794,8 +804,7 @@ __global__ void __launch_bounds__(256) xa_join(XaArgs p)
 		o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
 		l += sl[g];
 	}
-	const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-	xa_out4<KIND>(p, xa_orow(p, bh, r), 4 * li, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+	xa_out4<KIND>(p, xa_orow(p, bh, r), 4 * li, xa_over(o, l));
 }
 
 } /* namespace s3k */
@@ -961,7 +970,7 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 	const long long rows = (long long)d->Sq * a.G, bh = (long long)d->B * d->Hkv;
 	if (rows == 0 || bh == 0)
 		return (int)hipSuccess;
-	if (rows > 0x3FFFFFFFll || bh * parts > 0x7FFFFFFFll)
+	if (rows > 0x3FFFFFFFll)
 		return (int)hipErrorInvalidValue;
 	a.rows = (int)rows;
 	a.ns = parts;
@@ -972,7 +981,7 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 	hipStream_t st = (hipStream_t)stream;
 	if (path == S3K_XATTN_GENERIC) {
 		const long long blocks = (rows * bh + 3) / 4;
-		if (blocks > 0x7FFFFFFFll)
+		if (!s3k_launchable(blocks, 256))
 			return (int)hipErrorInvalidValue;
 		a.nrb = 0;
 		switch (d->kind) {
@@ -984,7 +993,7 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 	}
 	const XaShape s = xa_shape(d, path);
 	const long long nrb = (rows + s.rows - 1) / s.rows, blocks = nrb * bh * parts;
-	if (blocks > 0x7FFFFFFFll)
+	if (!s3k_launchable(blocks, 256))
 		return (int)hipErrorInvalidValue;
 	a.nrb = (int)nrb;
 	const int es = d->kind == S3K_F32 ? 4 : 2;

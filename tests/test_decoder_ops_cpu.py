@@ -170,3 +170,23 @@ def test_cross_attention_refusals():
     (dict(out=OK + 2), 1), (dict(H=0), 0), (dict(D=300), 0)])
 def test_cross_attention_path(kw, path):
     assert hip.load().sam3_hip_cross_attention_path(C.byref(cross(**kw))) == path
+
+
+def test_too_large_for_a_launch():
+    """More work-items than one launch takes, and more rows than the kernels
+    count, are refused before any launch."""
+    lib = hip.load()
+    big, over = 1 << 30, (1 << 30) + 1
+    for fn in (lib.sam3_hip_fp8_quantize, lib.sam3_hip_fp8_quantize_weight):
+        assert fn(abi.BF16, OK, 8, over, 8, OK, OK, None) == abi.EINVAL
+    assert lib.sam3_hip_fp8_quantize(abi.BF16, OK, 128, big, 128, OK, OK, None) == abi.EINVAL
+    assert lib.sam3_hip_fp8_quantize_weight(abi.BF16, OK, 1 << 22, big, 1 << 22, OK, OK, None) == abi.EINVAL
+    mm = lib.sam3_hip_matmul_fp8
+    for M, N in ((over, 8), (8, over), (big, big)):
+        for c in (abi.F32, abi.BF16):
+            assert mm(OK, OK, OK, OK, c, OK, M, N, 8, None, 0, None) == abi.EINVAL, (M, N, c)
+    lin = lib.sam3_hip_linear_fp8
+    assert lin(abi.BF16, OK, 8, OK, OK, abi.BF16, OK, 1, big, 8, None, 0, None, 0, None) == abi.EINVAL
+    assert norm_rope(B=1 << 16, S=1 << 16) == abi.EINVAL
+    p = cross(H=1 << 20, Hkv=1 << 20, Sq=1000, D=7)
+    assert lib.sam3_hip_cross_attention(C.byref(p), None, 0, None) == abi.EINVAL

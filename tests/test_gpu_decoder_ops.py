@@ -270,6 +270,18 @@ def test_matmul_fp8_large(c_dt, M, N, K, flags):
     assert (c[M] == 7.0).all()
 
 
+@pytest.mark.parametrize("c_dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("M,N,K,flags", [
+    (4400, 5003, 1100, hip.BIAS), (5600, 4104, 1100, hip.BIAS | hip.GELU), (4700, 5400, 1030, 0),
+    (5000, 5003, 1100, hip.BIAS | hip.GELU), (5600, 6000, 390, hip.BIAS), (333, 2004, 700, hip.BIAS),
+    (500, 1001, 700, hip.GELU), (2000, 3001, 300, hip.BIAS), (77, 1000, 4096, 0)])
+def test_matmul_fp8_many_tiles(c_dt, M, N, K, flags):
+    """More tiles than CUs, so that a workgroup takes several, with odd and
+    even numbers of blocks and ends inside tiles; and sizes between those
+    of the other tests, where the kernel changes."""
+    test_matmul_fp8_large(c_dt, M, N, K, flags)
+
+
 def test_matmul_fp8_k0_and_nan():
     c = torch.full((40, 9), 7.0, device="cuda")
     bias = torch.arange(9.0, device="cuda")
@@ -678,6 +690,34 @@ def test_cross_attention_infinite_scores(dt, path):
     check_cross(dt, q2, k, v, path=path, what="nan query")
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [
+    (1, 1, 1, 1100, 3000, 64), (1, 2, 1, 530, 2600, 256), (1, 1, 1, 1030, 2100, 16), (1, 4, 1, 300, 1700, 96),
+    (1, 1, 1, 1, 40000, 64), (1, 3, 3, 2, 9000, 24), (1, 1, 1, 1, 20001, 200)])
+def test_cross_attention_parts(dt, B, H, Hkv, Sq, Sk, D):
+    """Keys shared out: many rows and few, as many parts as are ever made,
+    and lengths that leave most parts without a key."""
+    q, k, v = qkv(B + H + Sq + Sk + D, dt, B, H, Hkv, Sq, Sk, D, 1.5)
+    assert hip.cross_attention_work(desc(dt, q, k, v, q)) > 0
+    check_cross(dt, q, k, v)
+    check_cross(dt, q, k, v, qn=[Sq - 1], kn=[70], what="short")
+    check_cross(dt, q, k, v, kn=[0], what="none")
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("path", [0, 3])
+@pytest.mark.parametrize("Sq,Sk", [(1, 90), (1, 6000), (40, 90), (200, 2000)])
+def test_cross_attention_no_weights_over_infinite_values(dt, path, Sq, Sk):
+    """Rows whose scores are all -inf are zeros whatever the values hold."""
+    q = torch.ones(1, Sq, 2, 64, dtype=TT[dt], device="cuda")
+    k = torch.full((1, Sk, 2, 64), -math.inf, dtype=TT[dt], device="cuda")
+    v = torch.full((1, Sk, 2, 64), math.inf, dtype=TT[dt], device="cuda")
+    v[:, ::2] = math.nan
+    out = torch.full_like(q, 7.0)
+    hip.cross_attention_dev(desc(dt, q, k, v, out), stream=stream(), path=path)
+    assert (out == 0).all()
+
+
 def test_cross_attention_long_cache():
     """Keys and values more than 2^32 bytes from their first one."""
     Sk, D, row = 600, 64, 1 << 22
@@ -752,6 +792,59 @@ def test_cross_attention_same_bits_every_time():
             out.zero_()
             hip.cross_attention_dev(p, stream=stream())
             assert torch.equal(out, first)
+
+
+# ------------------------------------------------------- calls side by side
+def test_calls_of_several_threads():
+    """Threads on streams of their own, all with the library's scratch, get
+    the results of calls one after the other."""
+    import threading
+
+    M, N, K = 90, 260, 900
+    jobs = []
+    for n in range(4):
+        g = rng(70 + n)
+        w8, sw = (t.cuda() for t in weights(g, N, K))
+        x = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda()
+        att = qkv(80 + n, abi.F16, 1, 4, 2, 1 + n, 5000, 64)
+        rot = torch.randn(1, 30, 2, 64, generator=g).cuda()
+        freq = torch.tensor([10000.0 ** (-i / 32) for i in range(32)], dtype=torch.float64, device="cuda")
+        jobs.append((x, w8, sw, att, rot, freq, torch.cuda.Stream()))
+
+    def run(job, st):
+        x, w8, sw, (q, k, v), rot, freq, _ = job
+        c = torch.empty(M, N, device="cuda")
+        o, r = torch.empty_like(q), torch.empty_like(rot)
+        hip.linear_fp8_dev(abi.BF16, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32, c.data_ptr(), M, N, K,
+                           stream=st)
+        hip.cross_attention_dev(desc(abi.F16, q, k, v, o), stream=st)
+        hip.norm_rope_dev(abi.F32, 1, 30, 64, 64, hip.ROPE_HALF,
+                          hip.Heads(rot.data_ptr(), r.data_ptr(), 2, 3840, 128, 64, 3840, 128, 64),
+                          freq=freq.data_ptr(), norm=True, stream=st)
+        return c, o, r
+
+    alone = [run(j, stream()) for j in jobs]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(jobs[n][-1]):
+                got[n] = [run(jobs[n], jobs[n][-1].cuda_stream) for _ in range(20)]
+                jobs[n][-1].synchronize()
+        except Exception as e:  # noqa: BLE001 - handed to the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for n in range(4):
+        for res in got[n]:
+            for a, b in zip(res, alone[n]):
+                assert torch.equal(a, b)
 
 
 # ------------------------------------------------------------- as one layer
