@@ -33,6 +33,7 @@ struct XaArgs {
 	float *part;            /* ns > 1: results of the parts              */
 };
 
+constexpr int XA_PARTS = 64; /* of a row's keys, at most */
 constexpr float XA_NONE = -3.402823466e38f; /* running maximum of no keys */
 
 __device__ __forceinline__ int xa_len(const int *lens, int b, int most)
@@ -488,6 +489,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 	constexpr int NT = DP / 16, VW = NT < 4 ? NT : 4, NU = NT / VW;
 	constexpr int UN = xa_f32_un(DP), KT = 16 * UN, NB = DP <= 64 ? 2 : 1;
 	constexpr int MV = RT * (NT * 4 + 2); /* values a lane merges */
+	/* long heads' scores in four sums: in one after the other 256 products
+	 * left results of 1440 keys 1.7e-6 off, in four 0.3e-6 (2 % more time) */
+	constexpr int NZ = DP >= 64 ? 4 : 1;
 	__shared__ float red[NWK > 1 ? (NWK - 1) * NWQ * MV * 64 : 1];
 	const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -575,14 +579,21 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 			float mt = -__builtin_inff();
 #pragma unroll
 			for (int n = 0; n < UN; ++n) {
-				s[n] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+				s3k_f32x4 z[NZ];
+#pragma unroll
+				for (int a = 0; a < NZ; ++a)
+					z[a] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 				for (int j = 0; j < NT; ++j) {
-					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].x, qf[t][j].x, s[n], 0, 0, 0);
-					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].y, qf[t][j].y, s[n], 0, 0, 0);
-					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].z, qf[t][j].z, s[n], 0, 0, 0);
-					s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].w, qf[t][j].w, s[n], 0, 0, 0);
+					z[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].x, qf[t][j].x, z[0], 0, 0, 0);
+					z[1 % NZ] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].y, qf[t][j].y, z[1 % NZ], 0, 0, 0);
+					z[2 % NZ] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].z, qf[t][j].z, z[2 % NZ], 0, 0, 0);
+					z[3 % NZ] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[P][n][j].w, qf[t][j].w, z[3 % NZ], 0, 0, 0);
 				}
+				if constexpr (NZ == 4)
+					s[n] = (z[0] + z[1]) + (z[2] + z[3]);
+				else
+					s[n] = z[0];
 				if (left < KT) {
 #pragma unroll
 					for (int e = 0; e < 4; ++e)
@@ -752,45 +763,45 @@ __global__ void __launch_bounds__(256) xa_join_many(XaArgs p)
 
 /*
  * The parts of a row joined, few rows: a workgroup per row, DP / 4 lanes with
- * four values each times NG groups, which share out the parts (one after the
- * other, 78 parts of a 40000-key row took 35 us of loads) and are added up
- * in LDS in order.
+ * four values each times 16 groups. A group takes every 16th part, all asked
+ * for at once (with 4 groups and loads one after the other 2 x 4 heads, 5000
+ * keys of 256 took 21.3 us, so 19.3), and the groups are added up in LDS in
+ * order.
  */
 template <int KIND, int DP>
-__global__ void __launch_bounds__(256) xa_join(XaArgs p)
+__global__ void __launch_bounds__(4 * DP) xa_join(XaArgs p)
 {
-	constexpr int L = DP / 4, NG = 256 / L;
+	constexpr int L = DP / 4, NG = 16, NP = XA_PARTS / NG;
+	static_assert(XA_PARTS <= 64, "a wave reads all maxima at once");
 	__shared__ float4 so[NG][L];
-	__shared__ float sm[4], sl[NG];
+	__shared__ float sl[NG];
 	const long long rows = (long long)(p.d.B * p.d.Hkv) * p.rows, row = blockIdx.x;
 	const int bh = (int)(row / p.rows), r = (int)(row - (long long)bh * p.rows);
 	if (r >= xa_len(p.d.q_len, bh / p.d.Hkv, p.d.Sq) * p.G)
 		return;
 	const float *pm = p.part + rows * p.ns * DP, *pl = pm + rows * p.ns;
-	const int li = threadIdx.x % L, grp = threadIdx.x / L;
-	/* this thread's first parts are asked for before the maximum is known */
-	const bool have = grp < p.ns;
-	float4 v = have ? *(const float4 *)(p.part + (grp * rows + row) * DP + 4 * li) : make_float4(0, 0, 0, 0);
-	float vm = have ? pm[grp * rows + row] : XA_NONE, vl = have ? pl[grp * rows + row] : 0.0f;
-	float m = XA_NONE;
-	for (int s = threadIdx.x; s < p.ns; s += 256)
-		m = fmaxf(m, pm[s * rows + row]);
-	m = wave_max_f32(m);
-	if ((threadIdx.x & 63) == 0)
-		sm[threadIdx.x >> 6] = m;
-	__syncthreads();
-	m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+	const int li = threadIdx.x % L, grp = threadIdx.x / L, lane = threadIdx.x & 63;
+	float4 v[NP];
+	float vm[NP], vl[NP];
+#pragma unroll
+	for (int i = 0; i < NP; ++i) {
+		const int s = grp + NG * i;
+		v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vm[i] = XA_NONE, vl[i] = 0.0f;
+		if (s < p.ns) {
+			const long long at = s * rows + row;
+			v[i] = *(const float4 *)(p.part + at * DP + 4 * li);
+			vm[i] = pm[at], vl[i] = pl[at];
+		}
+	}
+	const float m = wave_max_f32(lane < p.ns ? pm[lane * rows + row] : XA_NONE);
 	float l = 0.0f;
 	float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-	for (int s = grp; s < p.ns; s += NG) {
-		const float a = __builtin_amdgcn_exp2f(vm - m);
-		l = fmaf(vl, a, l);
-		o.x = fmaf(v.x, a, o.x), o.y = fmaf(v.y, a, o.y), o.z = fmaf(v.z, a, o.z), o.w = fmaf(v.w, a, o.w);
-		if (s + NG < p.ns) {
-			const long long at = (s + NG) * rows + row;
-			v = *(const float4 *)(p.part + at * DP + 4 * li);
-			vm = pm[at], vl = pl[at];
-		}
+#pragma unroll
+	for (int i = 0; i < NP; ++i) {
+		const float a = __builtin_amdgcn_exp2f(vm[i] - m);
+		l = fmaf(vl[i], a, l);
+		o.x = fmaf(v[i].x, a, o.x), o.y = fmaf(v[i].y, a, o.y);
+		o.z = fmaf(v[i].z, a, o.z), o.w = fmaf(v[i].w, a, o.w);
 	}
 	so[grp][li] = o;
 	if (li == 0)
@@ -798,8 +809,8 @@ __global__ void __launch_bounds__(256) xa_join(XaArgs p)
 	__syncthreads();
 	if (grp > 0)
 		return;
-	const int n = p.ns < NG ? p.ns : NG;
-	for (int g = 1; g < n; ++g) {
+#pragma unroll
+	for (int g = 1; g < NG; ++g) {
 		const float4 u = so[g][li];
 		o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
 		l += sl[g];
@@ -887,12 +898,12 @@ template <int KIND, int DP>
 int xa_joined(const XaArgs &a, hipStream_t st)
 {
 	const long long rows = (long long)a.d.B * a.d.Hkv * a.rows, per = 256 / (DP / 4);
-	/* 5184 rows of 12 parts: 15 us by lanes, 35 by workgroups; 16 rows of 78
-	 * parts 38 and 5 */
-	if (rows > 1024)
+	/* whole calls of 4000 keys, 256 rows of 64 values: 16.6 us by lanes, 11.9
+	 * by workgroups; 2048 of 256 46.0 and 45.8; 4096 of 256 51 and 56 */
+	if (rows > 2048)
 		hipLaunchKernelGGL((xa_join_many<KIND, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a);
 	else
-		hipLaunchKernelGGL((xa_join<KIND, DP>), dim3((unsigned)rows), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_join<KIND, DP>), dim3((unsigned)rows), dim3(4 * DP), 0, st, a);
 	return (int)hipGetLastError();
 }
 
@@ -950,8 +961,8 @@ extern "C" int s3k_xattn_parts(const struct s3k_xattn *d, int path)
 	const long long most = few ? (d->Sk >= 4 * step ? d->Sk / step : 1) : d->Sk / (4 * step);
 	if (parts > most)
 		parts = most;
-	if (parts > 64)
-		parts = 64;
+	if (parts > XA_PARTS)
+		parts = XA_PARTS;
 	return parts < 2 ? 1 : (int)parts;
 }
 

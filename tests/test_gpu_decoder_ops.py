@@ -692,7 +692,7 @@ def test_cross_attention_infinite_scores(dt, path):
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
 @pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [
-    (1, 1, 1, 1100, 3000, 64), (1, 2, 1, 530, 2600, 256), (1, 1, 1, 1030, 2100, 16), (1, 4, 1, 300, 1700, 96),
+    (1, 1, 1, 1100, 3000, 64), (1, 2, 1, 1100, 2600, 256), (1, 1, 1, 1030, 2100, 16), (1, 1, 1, 2100, 1100, 64), (1, 4, 1, 300, 1700, 96),
     (1, 1, 1, 1, 40000, 64), (1, 3, 3, 2, 9000, 24), (1, 1, 1, 1, 20001, 200)])
 def test_cross_attention_parts(dt, B, H, Hkv, Sq, Sk, D):
     """Keys shared out: many rows and few, as many parts as are ever made,
