@@ -492,6 +492,9 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 	/* long heads' scores in four sums: in one after the other 256 products
 	 * left results of 1440 keys 1.7e-6 off, in four 0.3e-6 (2 % more time) */
 	constexpr int NZ = DP >= 64 ? 4 : 1;
+	/* results and sums of weights in two where registers allow, for the same
+	 * reason (14418 keys in one part: 1.6e-6 off, so 1.2e-6; no more time) */
+	constexpr int NO = DP <= 64 ? 2 : 1;
 	__shared__ float red[NWK > 1 ? (NWK - 1) * NWQ * MV * 64 : 1];
 	const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -521,14 +524,18 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 	const float *K0 = (const float *)p.d.k + b * p.d.k_b + hk * p.d.k_h;
 	const float *V0 = (const float *)p.d.v + b * p.d.v_b + hk * p.d.v_h;
 
-	s3k_f32x4 o[RT][NT];
-	float m[RT], l[RT];
+	s3k_f32x4 os[NO][RT][NT];
+	float m[RT], ls[NO][RT];
 #pragma unroll
 	for (int t = 0; t < RT; ++t) {
-		m[t] = XA_NONE, l[t] = 0.0f;
+		m[t] = XA_NONE;
 #pragma unroll
-		for (int j = 0; j < NT; ++j)
-			o[t][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+		for (int a = 0; a < NO; ++a) {
+			ls[a][t] = 0.0f;
+#pragma unroll
+			for (int j = 0; j < NT; ++j)
+				os[a][t][j] = (s3k_f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+		}
 	}
 	float4 kf[NB][UN][NT];
 	float vf[NB][UN][4][NU][VW];
@@ -608,25 +615,28 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 			if (__any(mt > m[t] + XA_SLACK)) {
 				const float mn = fmaxf(m[t], mt), al = __builtin_amdgcn_exp2f(m[t] - mn);
 				m[t] = mn;
-				l[t] *= al;
 #pragma unroll
-				for (int j = 0; j < NT; ++j)
+				for (int a = 0; a < NO; ++a) {
+					ls[a][t] *= al;
 #pragma unroll
-					for (int e = 0; e < 4; ++e)
-						o[t][j][e] *= al;
+					for (int j = 0; j < NT; ++j)
+#pragma unroll
+						for (int e = 0; e < 4; ++e)
+							os[a][t][j][e] *= al;
+				}
 			}
 #pragma unroll
 			for (int n = 0; n < UN; ++n)
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const float pe = __builtin_amdgcn_exp2f(fmaf(s[n][e], p.c, -m[t]));
-					l[t] += pe;
+					ls[e % NO][t] += pe;
 #pragma unroll
 					for (int u = 0; u < NU; ++u)
 #pragma unroll
 						for (int w = 0; w < VW; ++w)
-							o[t][u * VW + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-								vf[P][n][e][u][w], pe, o[t][u * VW + w], 0, 0, 0);
+							os[e % NO][t][u * VW + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+								vf[P][n][e][u][w], pe, os[e % NO][t][u * VW + w], 0, 0, 0);
 				}
 		}
 	};
@@ -653,8 +663,17 @@ __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 			work(b1, tile + NWK);
 		}
 	}
+	s3k_f32x4 (&o)[RT][NT] = os[0];
+	float (&l)[RT] = ls[0];
 #pragma unroll
 	for (int t = 0; t < RT; ++t) {
+#pragma unroll
+		for (int a = 1; a < NO; ++a) {
+			l[t] += ls[a][t];
+#pragma unroll
+			for (int j = 0; j < NT; ++j)
+				o[t][j] += os[a][t][j];
+		}
 		l[t] += __shfl_xor(l[t], 16);
 		l[t] = at_sum_pair(l[t]);
 	}
