@@ -438,14 +438,16 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
  * stored 8 columns a lane: the groups' pieces of two tiles are exchanged
  * (v_permlane32_swap, v_permlane16_swap) so that groups 0 and 1 hold the
  * first tile and 2 and 3 the second, 64 bytes of a row together instead of
- * 32 by halves of 8.
+ * 32 by halves of 8. The largest tiles' rows of whole 128-byte lines go past
+ * the caches (PAST; 20736 x 4096 x 1024 114 us, through them 124); rows that
+ * share lines meet there (20736 x 2000 x 1000 62, past them 83).
  */
-template <int CK, int NT, int MT>
+template <int CK, bool PAST, int NT, int MT>
 __device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (&acc)[NT][MT], int m, int n,
 					      int g, int flags)
 {
 	if constexpr (CK != S3K_F32 && NT % 2 == 0) {
-		if (p.vec == 2 && n + 16 * NT <= p.N) {
+		if (p.vec >= 2 && n + 16 * NT <= p.N) {
 #pragma unroll
 			for (int i = 0; i < NT; i += 2) {
 				const float4 b0 = f8_bias4<CK>(p, n + 16 * i + 4 * g, flags);
@@ -463,9 +465,14 @@ __device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (
 						w[e] = q[0], w[2 + e] = q[1];
 					}
 					const s3k_u32x4 v = {w[0], w[1], w[2], w[3]};
-					if (m + 16 * j < p.M)
-						__builtin_nontemporal_store(v, (s3k_u32x4 *)((uint16_t *)p.c + (long long)(m + 16 * j) * p.N +
-											      n + 16 * i + 8 * g));
+					s3k_u32x4 *const at = (s3k_u32x4 *)((uint16_t *)p.c + (long long)(m + 16 * j) * p.N +
+									    n + 16 * i + 8 * g);
+					if (m + 16 * j < p.M) {
+						if constexpr (PAST)
+							__builtin_nontemporal_store(v, at);
+						else
+							*at = v;
+					}
 				}
 			}
 			return;
@@ -511,14 +518,16 @@ __device__ __forceinline__ void f8_place(const F8Args &p, unsigned id, int &mt, 
  * block of both operands (rows of 8 16-byte chunks, swizzled) and the
  * rows' scales; two stages in a ring, filled by direct-to-LDS loads a
  * block ahead, over the end of a tile into the next one where a workgroup
- * takes several (20736 x 4096 x 1024 with GELU: 112 us, a workgroup for
- * each tile 117). KS such groups of waves, each with stages of its own, take
+ * takes several (MANY; 20736 x 4096 x 1024 with GELU: 112 us, a workgroup
+ * for each tile 117; smaller tiles, more than one on a CU, overlap by
+ * themselves, and were 5 % slower with it). KS such groups of waves, each with stages of its own, take
  * every KS-th block and are added up in LDS: for few tiles, whose blocks
  * one after the other would leave most CUs idle.
  */
-template <int CK, int BM, int BN, int WM, int WN, int KS>
+template <int CK, int BM, int BN, int WM, int WN, int KS, bool PAST>
 __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) f8_tile(F8Args p, int flags)
 {
+	constexpr bool MANY = WM * WN > 4; /* tiles of a workgroup */
 	constexpr int NST = 2, NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
 	constexpr int WB = BN * F8_BLK, AB = BM * F8_BLK, SB = NW * 256, STAGE = WB + AB + SB;
 	constexpr int WI = BN / 8, AI = BM / 8; /* 1 KiB loads per stage */
@@ -576,7 +585,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 		issue(t, ks, 0);
 	unsigned slot = 0;
 	wait_vm<0>();
-	for (unsigned tile = blockIdx.x; tile < total; tile += gridDim.x) {
+	unsigned tile = blockIdx.x;
+	do {
 		/* where this tile lies; m0 and n0 move on to the next one at its end */
 		const int tm = m0, tn = n0 + wn * (BN / WN);
 		const float *swp = p.sw + (long long)(tn / F8_BLK) * p.KB;
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 		for (int k0 = 0; k0 < p.KB; k0 += KS) {
 			const int kb = k0 + ks;
 			int ask = kb + KS;
-			if (k0 + KS >= p.KB && tile + gridDim.x < total) {
+			if (MANY && k0 + KS >= p.KB && tile + gridDim.x < total) {
 				/* the next tile's first block, before this one's is stored */
 				place(tile + gridDim.x);
 				ask = ks;
@@ -663,8 +673,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 							acc[i][j][r] += v[r];
 					}
 		}
-		f8_tile_store<CK, NT, MT>(p, acc, tm + wm * (BM / WM) + l16, tn, g, flags);
-	}
+		f8_tile_store<CK, PAST, NT, MT>(p, acc, tm + wm * (BM / WM) + l16, tn, g, flags);
+		tile += gridDim.x;
+	} while (MANY && tile < total);
 }
 
 /*
@@ -830,7 +841,15 @@ int f8_tile_run(F8Args &a, int flags, hipStream_t st)
 	const long long grid = WM * WN > 4 && a.KB > 0 && blocks > 256 ? 256 : blocks;
 	if (blocks > 0x7FFFFFFFll || !s3k_launchable(grid, 64 * WM * WN * KS))
 		return (int)hipErrorInvalidValue;
-	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS>), dim3((unsigned)grid), dim3(64 * WM * WN * KS), 0, st, a, flags);
+	const dim3 g((unsigned)grid), wg(64 * WM * WN * KS);
+	if constexpr (WM * WN > 4) {
+		/* rows of whole lines */
+		if (a.N % 64 == 0 && (uintptr_t)a.c % 128 == 0) {
+			hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS, true>), g, wg, 0, st, a, flags);
+			return (int)hipGetLastError();
+		}
+	}
+	hipLaunchKernelGGL((f8_tile<CK, BM, BN, WM, WN, KS, false>), g, wg, 0, st, a, flags);
 	return (int)hipGetLastError();
 }
 
@@ -855,19 +874,19 @@ int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 
 /*
  * The kernel of a product, by an estimate of each one's time from its grid.
- * Measured (bf16, 10 row counts from 24 to 20736 by five N x K, and 8192^3),
- * the tile kernels take, in us, for a block of k with one workgroup on a CU
- * and with all that fit, and for the rest of a tile; a round is one
+ * Measured (bf16, 12 row counts from 24 to 20736 by seven N x K, and
+ * 8192^3), the tile kernels take, in us, for a block of k with one workgroup
+ * on a CU and with all that fit, and for the rest of a tile; a round is one
  * workgroup in every place. The few-rows kernels are linear in their
- * workgroups. The kernel it takes was at most 12 % behind the quickest, 1 %
+ * workgroups. The kernel it takes was at most 4 % behind the quickest, 0.1 %
  * in the mean. Examples, us:
  *
  *     M x N x K            64  64/2  64/4   128  192x256  256  rows 1  2
- *     77 x 1024 x 4096   16.5  12.1  10.4  25.4    40.2  48.1   5.9   4.2
- *     400 x 1024 x 4096  16.9  12.4  10.8  26.0    41.4  49.0  17.6  13.0
- *     1369 x 4096 x 1024 14.5  18.2  27.0  12.3    15.5  17.9  65    71
- *     20736 x 4096 x 1024 165   209   363   121     106   115  931  1030
- *     8192^3              850               555     545   470
+ *     77 x 1024 x 4096   16.0  11.1   9.7  26.1    40.0  47.9   6.0   4.3
+ *     400 x 1024 x 4096  16.5  11.7  10.4  26.5    41.2  48.8  17.4  13.1
+ *     1369 x 4096 x 1024 14.4  17.7  25.5  13.7    16.9  19.7  65    71
+ *     20736 x 4096 x 1024 163   206   339   118     109   105   942  1031
+ *     8192^3              842               570     556   459
  *
  * (64/2: two groups of waves share out the blocks.) The two largest tiles
  * are not built for f32 outputs, whose wider operands spill there.
@@ -879,8 +898,8 @@ struct F8Cost {
 	double one, full, rest;
 };
 const F8Cost f8_costs[F8_ROWS1] = {
-	{64, 64, 1, 4, 0.35, 0.82, 1.0},   {64, 64, 2, 2, 0.61, 0.97, 1.2},   {64, 64, 4, 1, 0.95, 0.95, 1.8},
-	{128, 128, 1, 2, 0.87, 1.22, 1.9}, {192, 256, 1, 1, 1.63, 1.63, 3.9}, {256, 256, 1, 1, 1.60, 1.60, 8.4},
+	{64, 64, 1, 4, 0.33, 0.84, 1.0},   {64, 64, 2, 2, 0.54, 0.97, 1.2},   {64, 64, 4, 1, 0.88, 1.07, 1.6},
+	{128, 128, 1, 2, 0.86, 1.15, 2.1}, {192, 256, 1, 1, 1.42, 1.28, 4.7}, {256, 256, 1, 1, 1.43, 1.35, 8.1},
 };
 
 double f8_estimate(int kernel, int M, int N, int KB)
@@ -888,8 +907,8 @@ double f8_estimate(int kernel, int M, int N, int KB)
 	if (kernel >= F8_ROWS1) {
 		const int mt = kernel == F8_ROWS1 ? 1 : 2;
 		const double wgs = (double)((N + 15ll) / 16) * ((M + 16ll * mt - 1) / (16 * mt));
-		return mt == 1 ? 2.4 + 0.012 * KB + wgs * (0.27e-3 * KB + 0.45e-3)
-			       : 2.3 + 0.029 * KB + wgs * (0.30e-3 * KB + 2.8e-3);
+		return mt == 1 ? 2.4 + 0.004 * KB + wgs * (0.35e-3 * KB + 0.2e-3)
+			       : 2.35 + 0.027 * KB + wgs * (0.31e-3 * KB + 2.5e-3);
 	}
 	const F8Cost &c = f8_costs[kernel];
 	const double tiles = (double)((M + c.bm - 1ll) / c.bm) * ((N + c.bn - 1ll) / c.bn), its = (KB + c.ks - 1) / c.ks;
