@@ -828,8 +828,8 @@ __global__ void __launch_bounds__(4 * DP) xa_join(XaArgs p)
 	__syncthreads();
 	if (grp > 0)
 		return;
-#pragma unroll
-	for (int g = 1; g < NG; ++g) {
+	const int n = p.ns < NG ? p.ns : NG;
+	for (int g = 1; g < n; ++g) {
 		const float4 u = so[g][li];
 		o.x += u.x, o.y += u.y, o.z += u.z, o.w += u.w;
 		l += sl[g];
