@@ -100,18 +100,25 @@ struct F8Raw {
 	uint4 v[N];
 };
 
-/* Values i..i+7 at p, those at and past `left` zero. vec: 16-byte aligned */
+/* Values i..i+7 at p as whole loads: memory takes them at any element's
+ * address (1222 x 6503 f16 quantized in 6.7 us, one value at a time 11.2). */
 template <int KIND>
-__device__ __forceinline__ F8Raw<KIND> f8_load8(const void *p, long long i, int left, int vec)
+__device__ __forceinline__ F8Raw<KIND> f8_whole8(const void *p, long long i)
 {
 	F8Raw<KIND> r;
-	if (vec && left >= 8) {
-		const uint4 *q = (const uint4 *)((const char *)p + i * (KIND == S3K_F32 ? 4 : 2));
 #pragma unroll
-		for (int j = 0; j < F8Raw<KIND>::N; ++j)
-			r.v[j] = q[j];
-		return r;
-	}
+	for (int j = 0; j < F8Raw<KIND>::N; ++j)
+		__builtin_memcpy(&r.v[j], (const char *)p + i * (KIND == S3K_F32 ? 4 : 2) + 16 * j, 16);
+	return r;
+}
+
+/* Values i..i+7 at p, those at and past `left` zero. */
+template <int KIND>
+__device__ __forceinline__ F8Raw<KIND> f8_load8(const void *p, long long i, int left)
+{
+	if (left >= 8)
+		return f8_whole8<KIND>(p, i);
+	F8Raw<KIND> r;
 	uint32_t w[4 * F8Raw<KIND>::N];
 #pragma unroll
 	for (int j = 0; j < 4 * F8Raw<KIND>::N; ++j) {
@@ -132,7 +139,7 @@ __device__ __forceinline__ F8Raw<KIND> f8_load8(const void *p, long long i, int 
 	return r;
 }
 
-/* Values i..i+7 at p, 16-byte aligned, or zeros. */
+/* Values i..i+7 at p, or zeros. */
 template <int KIND>
 __device__ __forceinline__ F8Raw<KIND> f8_chunk(const void *p, long long i, bool in)
 {
@@ -140,12 +147,8 @@ __device__ __forceinline__ F8Raw<KIND> f8_chunk(const void *p, long long i, bool
 #pragma unroll
 	for (int j = 0; j < F8Raw<KIND>::N; ++j)
 		r.v[j] = make_uint4(0, 0, 0, 0);
-	if (in) {
-		const uint4 *q = (const uint4 *)((const char *)p + i * (KIND == S3K_F32 ? 4 : 2));
-#pragma unroll
-		for (int j = 0; j < F8Raw<KIND>::N; ++j)
-			r.v[j] = q[j];
-	}
+	if (in)
+		r = f8_whole8<KIND>(p, i);
 	return r;
 }
 
@@ -299,7 +302,7 @@ __device__ __forceinline__ float f8_group(const F8Raw<KIND> (&r)[C], uint2 (&q)[
  */
 template <int KIND>
 __global__ void __launch_bounds__(256) f8_quant_rows(const void *x, long long ldx, int rows, int K,
-						      int KB, int vec, uint8_t *q, float *scale)
+						      int KB, uint8_t *q, float *scale)
 {
 	const long long g = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
 	const int li = threadIdx.x & 15;
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(256) f8_quant_rows(const void *x, long long ld
 		return;
 	const int m = (int)(g / KB), kb = (int)(g - (long long)m * KB);
 	const int k0 = kb * F8_BLK + li * 8;
-	const F8Raw<KIND> r[1] = {f8_load8<KIND>(x, m * ldx + k0, K - k0, vec)};
+	const F8Raw<KIND> r[1] = {f8_load8<KIND>(x, m * ldx + k0, K - k0)};
 	uint2 o[1];
 	const float up = f8_group<KIND, 1, 15>(r, o);
 	*(uint2 *)(q + g * F8_BLK + li * 8) = o[0];
@@ -355,9 +358,6 @@ struct F8Args {
 	const void *bias;
 	int M, N, KB;
 	int nmt, nnt;           /* tiles along M and N                       */
-	int vec;                /* columns of C stored together: 1 four, 2 also
-				 * eight of 16 bits                          */
-	int bvec;               /* four values of the bias loaded together   */
 	/* fused quantization: x in place of a, sa */
 	const void *x;
 	long long ldx;
@@ -369,10 +369,13 @@ template <int CK>
 __device__ __forceinline__ float4 f8_bias4(const F8Args &p, int n, int flags)
 {
 	float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-	if ((flags & S3K_EPI_BIAS) && p.bvec && n + 3 < p.N) {
-		if constexpr (CK == S3K_F32)
-			return *(const float4 *)((const float *)p.bias + n);
-		const uint2 w = *(const uint2 *)((const uint16_t *)p.bias + n);
+	if ((flags & S3K_EPI_BIAS) && n + 3 < p.N) {
+		if constexpr (CK == S3K_F32) {
+			__builtin_memcpy(b, (const float *)p.bias + n, 16);
+			return make_float4(b[0], b[1], b[2], b[3]);
+		}
+		uint2 w;
+		__builtin_memcpy(&w, (const uint16_t *)p.bias + n, 8);
 		if constexpr (CK == S3K_BF16)
 			return make_float4(bf16_to_f32(w.x & 0xFFFFu), bf16_to_f32(w.x >> 16),
 					   bf16_to_f32(w.y & 0xFFFFu), bf16_to_f32(w.y >> 16));
@@ -417,13 +420,14 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
 			x[e] = gelu_tanh(x[e]);
 	}
 	const long long at = (long long)m * p.N + n;
-	if (p.vec && n + 3 < p.N) {
-		if constexpr (CK == S3K_F32)
-			*(float4 *)((float *)p.c + at) = make_float4(x[0], x[1], x[2], x[3]);
-		else if constexpr (CK == S3K_BF16)
-			*(uint2 *)((uint16_t *)p.c + at) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-		else
-			*(uint2 *)((uint16_t *)p.c + at) = make_uint2(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]));
+	if (n + 3 < p.N) {
+		if constexpr (CK == S3K_F32) {
+			__builtin_memcpy((float *)p.c + at, x, 16);
+		} else {
+			const uint2 w = CK == S3K_BF16 ? make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]))
+						       : make_uint2(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]));
+			__builtin_memcpy((uint16_t *)p.c + at, &w, 8);
+		}
 		return;
 	}
 #pragma unroll
@@ -434,8 +438,8 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
 
 /*
  * A wave's NT x MT tiles: row m + 16 j, columns n + 16 i + 4 g + 0..3 in
- * acc[i][j] of lane group g. 16-bit outputs with whole 16-byte rows are
- * stored 8 columns a lane: the groups' pieces of two tiles are exchanged
+ * acc[i][j] of lane group g. 16-bit outputs are stored 8 columns a lane, at
+ * any element's address (20000 x 4001 x 500 106 us, one at a time 156): the groups' pieces of two tiles are exchanged
  * (v_permlane32_swap, v_permlane16_swap) so that groups 0 and 1 hold the
  * first tile and 2 and 3 the second, 64 bytes of a row together instead of
  * 32 by halves of 8. The largest tiles' rows of whole 128-byte lines go past
@@ -447,7 +451,7 @@ __device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (
 					      int g, int flags)
 {
 	if constexpr (CK != S3K_F32 && NT % 2 == 0) {
-		if (p.vec >= 2 && n + 16 * NT <= p.N) {
+		if (n + 16 * NT <= p.N) {
 #pragma unroll
 			for (int i = 0; i < NT; i += 2) {
 				const float4 b0 = f8_bias4<CK>(p, n + 16 * i + 4 * g, flags);
@@ -465,13 +469,12 @@ __device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (
 						w[e] = q[0], w[2 + e] = q[1];
 					}
 					const s3k_u32x4 v = {w[0], w[1], w[2], w[3]};
-					s3k_u32x4 *const at = (s3k_u32x4 *)((uint16_t *)p.c + (long long)(m + 16 * j) * p.N +
-									    n + 16 * i + 8 * g);
+					uint16_t *const at = (uint16_t *)p.c + (long long)(m + 16 * j) * p.N + n + 16 * i + 8 * g;
 					if (m + 16 * j < p.M) {
 						if constexpr (PAST)
-							__builtin_nontemporal_store(v, at);
+							__builtin_nontemporal_store(v, (s3k_u32x4 *)at);
 						else
-							*at = v;
+							__builtin_memcpy(at, &v, 16);
 					}
 				}
 			}
@@ -692,10 +695,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
  * XK >= 0 (MT = 1): x of that type is quantized in registers on the way: a
  * lane holds 32 values of row lane & 15, the group's other three quarters
  * are 16, 32 and 48 lanes on. Every workgroup repeats that, which one
- * launch less pays for up to 16 rows; x has to be 16-byte aligned and K a
- * multiple of 8 (the checks of other cases cost more in instruction fetches
- * than the launch). XK < 0: quantized rows, 16 MT of
- * them from blockIdx.y on.
+ * launch less pays for up to 16 rows; K has to be a multiple of 8 (the
+ * checks of other cases cost more in instruction fetches than the launch).
+ * XK < 0: quantized rows, 16 MT of them from blockIdx.y on.
  */
 template <int XK, int CK, int MT, int NWV>
 __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
@@ -965,20 +967,11 @@ int f8_rows_ck(F8Args &a, int ck, int flags, hipStream_t st)
 	return (int)hipErrorInvalidValue;
 }
 
-bool vec16(const void *p, long long ld, int kind)
-{
-	return (uintptr_t)p % 16 == 0 && ld % (kind == S3K_F32 ? 4 : 8) == 0;
-}
-
-F8Args f8_args(const void *w, const float *sw, void *c, int ck, int M, int N, int K, const void *bias)
+F8Args f8_args(const void *w, const float *sw, void *c, int M, int N, int K, const void *bias)
 {
 	F8Args a = {};
 	a.w = (const uint8_t *)w, a.sw = sw, a.c = c, a.bias = bias;
 	a.M = M, a.N = N, a.K = K, a.KB = (K + F8_BLK - 1) / F8_BLK;
-	a.vec = N % 4 == 0 && (uintptr_t)c % (ck == S3K_F32 ? 16 : 8) == 0;
-	if (N % 8 == 0 && (uintptr_t)c % 16 == 0)
-		a.vec = 2;
-	a.bvec = bias && (uintptr_t)bias % (ck == S3K_F32 ? 16 : 8) == 0;
 	return a;
 }
 
@@ -994,10 +987,9 @@ extern "C" int s3k_fp8_quantize(int kind, const void *x, long long ldx, int rows
 	if (!s3k_launchable(blocks, 256))
 		return (int)hipErrorInvalidValue;
 	hipStream_t st = (hipStream_t)stream;
-	const int vec = vec16(x, ldx, kind);
 #define F8_Q(KIND)                                                                                  \
 	hipLaunchKernelGGL((f8_quant_rows<KIND>), dim3((unsigned)blocks), dim3(256), 0, st, x, ldx, rows, K, \
-			   KB, vec, (uint8_t *)q, scale)
+			   KB, (uint8_t *)q, scale)
 	switch (kind) {
 	case S3K_F32: F8_Q(S3K_F32); break;
 	case S3K_F16: F8_Q(S3K_F16); break;
@@ -1027,7 +1019,7 @@ extern "C" int s3k_fp8_matmul(const void *q, const float *sa, const void *w, con
 {
 	if (M == 0 || N == 0)
 		return (int)hipSuccess;
-	F8Args a = f8_args(w, sw, c, ck, M, N, K, bias);
+	F8Args a = f8_args(w, sw, c, M, N, K, bias);
 	a.a = (const uint8_t *)q, a.sa = sa;
 	switch (ck) {
 	case S3K_F32: return f8_product<S3K_F32>(a, flags, (hipStream_t)stream);
@@ -1037,9 +1029,9 @@ extern "C" int s3k_fp8_matmul(const void *q, const float *sa, const void *w, con
 	return (int)hipErrorInvalidValue;
 }
 
-extern "C" int s3k_fp8_rows_ok(int xk, const void *x, long long ldx, int M, int K)
+extern "C" int s3k_fp8_rows_ok(int M, int K)
 {
-	return M <= S3K_FP8_ROWS_MAX && K % 8 == 0 && vec16(x, ldx, xk);
+	return M <= S3K_FP8_ROWS_MAX && K % 8 == 0;
 }
 
 extern "C" int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,
@@ -1047,9 +1039,9 @@ extern "C" int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w,
 {
 	if (M == 0 || N == 0)
 		return (int)hipSuccess;
-	if (!s3k_fp8_rows_ok(xk, x, ldx, M, K))
+	if (!s3k_fp8_rows_ok(M, K))
 		return (int)hipErrorInvalidValue;
-	F8Args a = f8_args(w, sw, c, ck, M, N, K, bias);
+	F8Args a = f8_args(w, sw, c, M, N, K, bias);
 	a.x = x, a.ldx = ldx;
 	switch (xk) {
 	case S3K_F32: return f8_rows_ck<S3K_F32>(a, ck, flags, (hipStream_t)stream);

@@ -167,7 +167,7 @@ enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, c
 	/* Every workgroup quantizes all of x again: with more than 256 blocks of
 	 * it a launch of its own is quicker (16 x 4096 x 4096 6.7 us, inside 7.8;
 	 * 8 x 4096 x 4096 6.4 and 6.3; 16 x 1024 x 1024 5.2 and 3.6). */
-	if (s3k_fp8_rows_ok(x_dtype, x, ldx, M, K) &&
+	if (s3k_fp8_rows_ok(M, K) &&
 	    ((long long)M * ((K + 127) / 128) <= 256 || (!work && captured(stream))))
 		return launched(s3k_fp8_rows(x_dtype, x, ldx, w, w_scale, c_dtype, c, M, N, K, bias, flags,
 					    stream),
