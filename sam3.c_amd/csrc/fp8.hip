@@ -152,6 +152,27 @@ __device__ __forceinline__ F8Raw<KIND> f8_chunk(const void *p, long long i, bool
 	return r;
 }
 
+/* r without its first s values (0 to 7), zeros behind. */
+template <int KIND>
+__device__ __forceinline__ void f8_drop(F8Raw<KIND> &r, int s)
+{
+	constexpr int N = 4 * F8Raw<KIND>::N, PER = 8 / N; /* words, values of one */
+	uint32_t w[N];
+	__builtin_memcpy(w, r.v, sizeof(w));
+#pragma unroll
+	for (int n = 4; n >= PER; n >>= 1)
+#pragma unroll
+		for (int i = 0; i < N; ++i)
+			if (s & n)
+				w[i] = i + n / PER < N ? w[i + n / PER < N ? i + n / PER : 0] : 0u;
+	if (PER == 2 && (s & 1)) {
+#pragma unroll
+		for (int i = 0; i < N; ++i)
+			w[i] = w[i] >> 16 | (i + 1 < N ? w[i + 1 < N ? i + 1 : 0] << 16 : 0u);
+	}
+	__builtin_memcpy(r.v, w, sizeof(w));
+}
+
 typedef unsigned short f8_us2 __attribute__((ext_vector_type(2)));
 
 /* The larger of two keys: magnitudes as the bits of their type without the
@@ -439,10 +460,10 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
 /*
  * A wave's NT x MT tiles: row m + 16 j, columns n + 16 i + 4 g + 0..3 in
  * acc[i][j] of lane group g. 16-bit outputs are stored 8 columns a lane, at
- * any element's address (20000 x 4001 x 500 106 us, one at a time 156): the groups' pieces of two tiles are exchanged
- * (v_permlane32_swap, v_permlane16_swap) so that groups 0 and 1 hold the
- * first tile and 2 and 3 the second, 64 bytes of a row together instead of
- * 32 by halves of 8. The largest tiles' rows of whole 128-byte lines go past
+ * any element's address (20000 x 4001 x 500 106 us, one at a time 156): the
+ * groups' pieces of two tiles are exchanged (v_permlane32_swap,
+ * v_permlane16_swap) so that groups 0 and 1 hold the first tile and 2 and 3
+ * the second, 64 bytes of a row together instead of 32 by halves of 8. The largest tiles' rows of whole 128-byte lines go past
  * the caches (PAST; 20736 x 4096 x 1024 114 us, through them 124); rows that
  * share lines meet there (20736 x 2000 x 1000 62, past them 83).
  */
@@ -695,11 +716,12 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
  * XK >= 0 (MT = 1): x of that type is quantized in registers on the way: a
  * lane holds 32 values of row lane & 15, the group's other three quarters
  * are 16, 32 and 48 lanes on. Every workgroup repeats that, which one
- * launch less pays for up to 16 rows; K has to be a multiple of 8 (the
- * checks of other cases cost more in instruction fetches than the launch).
+ * launch less pays for up to 16 rows. The last values of a K that is no
+ * multiple of 8 (TAIL) are read as the row's last 8 (K is at least 8) and
+ * moved down; the code for it costs other lengths 0.15 to 0.5 us.
  * XK < 0: quantized rows, 16 MT of them from blockIdx.y on.
  */
-template <int XK, int CK, int MT, int NWV>
+template <int XK, int CK, int MT, int NWV, bool TAIL>
 __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 {
 	static_assert(XK < 0 || MT == 1, "quantized on the way: 16 rows");
@@ -754,11 +776,11 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 			for (int c = 0; c < 4; ++c) {
 				/* bytes 16 g and 64 + 16 g onward, as the weights' */
 				const int k = k0 + 64 * (c >> 1) + 8 * (c & 1);
-				x[S][c] = f8_chunk<XK>(p.x, l16 * p.ldx + k, l16 < p.M && k < p.K);
+				x[S][c] = f8_chunk<XK>(p.x, l16 * p.ldx + (TAIL ? min(k, p.K - 8) : k), l16 < p.M && k < p.K);
 			}
 		}
 	};
-	auto work = [&](auto slot) __attribute__((always_inline)) {
+	auto work = [&](auto slot, int kb) __attribute__((always_inline)) {
 		constexpr int S = decltype(slot)::value;
 		const unsigned at = mine + S * SLOT;
 		const f8_i8 fw = f8_join(lds_rd16(at + rd0, 0), lds_rd16(at + rd1, 0));
@@ -772,6 +794,13 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 			} else {
 				/* an infinity or NaN makes all of its row's results NaN,
 				 * whatever the group's other values become */
+				if (TAIL && kb == p.KB - 1) {
+#pragma unroll
+					for (int c = 0; c < 4; ++c) {
+						const int k = kb * F8_BLK + 16 * g + 64 * (c >> 1) + 8 * (c & 1);
+						f8_drop<XK>(x[S][c], k < p.K ? max(k - (p.K - 8), 0) : 0);
+					}
+				}
 				const float amax = f8_group_max<XK, 4, 48>(x[S]);
 				const float up = pow2f(f8_exp_of(amax));
 				uint2 q[4];
@@ -797,9 +826,9 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 	for (int kb = wave; kb < p.KB; kb += 2 * NWV) {
 		wait_vm<0>(); /* both blocks: the compiler does not see these loads */
 		__builtin_amdgcn_sched_barrier(0);
-		work(even);
+		work(even, kb);
 		if (kb + NWV < p.KB)
-			work(odd);
+			work(odd, kb + NWV);
 		if (kb + 2 * NWV < p.KB) {
 			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); /* the slots are read */
 			load(even, kb + 2 * NWV);
@@ -855,7 +884,7 @@ int f8_tile_run(F8Args &a, int flags, hipStream_t st)
 	return (int)hipGetLastError();
 }
 
-template <int XK, int CK, int MT>
+template <int XK, int CK, int MT, bool TAIL>
 int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 {
 	const unsigned mb = (unsigned)((a.M + 16 * MT - 1) / (16 * MT)); /* M is small */
@@ -866,11 +895,11 @@ int f8_rows_go(F8Args &a, int flags, hipStream_t st)
 	 * tiles, for their LDS) */
 	if constexpr (MT == 1) {
 		if (a.KB > 8) {
-			hipLaunchKernelGGL((f8_rows<XK, CK, MT, 16>), dim3(nb, mb), dim3(1024), 0, st, a, flags);
+			hipLaunchKernelGGL((f8_rows<XK, CK, MT, 16, TAIL>), dim3(nb, mb), dim3(1024), 0, st, a, flags);
 			return (int)hipGetLastError();
 		}
 	}
-	hipLaunchKernelGGL((f8_rows<XK, CK, MT, 8>), dim3(nb, mb), dim3(512), 0, st, a, flags);
+	hipLaunchKernelGGL((f8_rows<XK, CK, MT, 8, TAIL>), dim3(nb, mb), dim3(512), 0, st, a, flags);
 	return (int)hipGetLastError();
 }
 
@@ -950,19 +979,25 @@ int f8_product(F8Args &a, int flags, hipStream_t st)
 		if constexpr (CK != S3K_F32)
 			return f8_tile_run<CK, 256, 256, 4, 2, 1>(a, flags, st);
 		break;
-	case F8_ROWS1: return f8_rows_go<-1, CK, 1>(a, flags, st);
-	case F8_ROWS2: return f8_rows_go<-1, CK, 2>(a, flags, st);
+	case F8_ROWS1: return f8_rows_go<-1, CK, 1, false>(a, flags, st);
+	case F8_ROWS2: return f8_rows_go<-1, CK, 2, false>(a, flags, st);
 	}
 	return f8_tile_run<CK, 64, 64, 2, 2, 1>(a, flags, st);
+}
+
+template <int XK, int CK>
+int f8_rows_x(F8Args &a, int flags, hipStream_t st)
+{
+	return a.K % 8 ? f8_rows_go<XK, CK, 1, true>(a, flags, st) : f8_rows_go<XK, CK, 1, false>(a, flags, st);
 }
 
 template <int XK>
 int f8_rows_ck(F8Args &a, int ck, int flags, hipStream_t st)
 {
 	switch (ck) {
-	case S3K_F32: return f8_rows_go<XK, S3K_F32, 1>(a, flags, st);
-	case S3K_F16: return f8_rows_go<XK, S3K_F16, 1>(a, flags, st);
-	case S3K_BF16: return f8_rows_go<XK, S3K_BF16, 1>(a, flags, st);
+	case S3K_F32: return f8_rows_x<XK, S3K_F32>(a, flags, st);
+	case S3K_F16: return f8_rows_x<XK, S3K_F16>(a, flags, st);
+	case S3K_BF16: return f8_rows_x<XK, S3K_BF16>(a, flags, st);
 	}
 	return (int)hipErrorInvalidValue;
 }
@@ -1031,7 +1066,7 @@ extern "C" int s3k_fp8_matmul(const void *q, const float *sa, const void *w, con
 
 extern "C" int s3k_fp8_rows_ok(int M, int K)
 {
-	return M <= S3K_FP8_ROWS_MAX && K % 8 == 0;
+	return M <= S3K_FP8_ROWS_MAX && (K == 0 || K >= 8);
 }
 
 extern "C" int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,

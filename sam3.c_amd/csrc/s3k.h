@@ -444,7 +444,7 @@ int s3k_fp8_quantize_weight(int kind, const void *w, long long ldw, int N, int K
 int s3k_fp8_matmul(const void *q, const float *sa, const void *w, const float *sw, int ck,
 		   void *c, int M, int N, int K, const void *bias, int flags, void *stream);
 /* x of up to S3K_FP8_ROWS_MAX rows, quantized inside the product's kernel,
- * where s3k_fp8_rows_ok (K a multiple of 8) */
+ * where s3k_fp8_rows_ok (K of 8 at least, or 0) */
 #define S3K_FP8_ROWS_MAX 16
 int s3k_fp8_rows_ok(int M, int K);
 int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,
