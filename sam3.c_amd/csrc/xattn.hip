@@ -28,6 +28,7 @@ struct XaArgs {
 	int G, rows;            /* query heads per key head; Sq * G          */
 	int nrb, ns;            /* row blocks per (b, h'); parts of the keys */
 	int run;                /* key heads kept on one XCD (xa_place)      */
+	int sort;               /* sequences of most keys first (xa_place)   */
 	float c;                /* scale * log2(e)                           */
 	int ovec;               /* 4 values of an output row stored together */
 	float *part;            /* ns > 1: results of the parts              */
@@ -48,7 +49,9 @@ __device__ __forceinline__ int xa_len(const int *lens, int b, int most)
  * round-robin. The row blocks that read the same keys get ids of one
  * residue mod 8 and share an XCD's L2, and so do p.run key heads whose rows
  * lie together in less than 256 bytes: apart, two XCDs each fetched the
- * same lines (16 x 8 heads of 16 f32, 5184 keys: 34 us, together 26). */
+ * same lines (16 x 8 heads of 16 f32, 5184 keys: 34 us, together 26). With
+ * p.sort the sequences of most keys go first, so that the last workgroups to
+ * run are short ones. */
 __device__ __forceinline__ void xa_place(const XaArgs &p, unsigned id, int &bh, int &part, int &rb)
 {
 	const unsigned runs = (unsigned)(p.d.Hkv / p.run), units = (unsigned)(p.d.B * p.ns) * runs;
@@ -66,7 +69,18 @@ __device__ __forceinline__ void xa_place(const XaArgs &p, unsigned id, int &bh, 
 	const int hk = (int)(u % runs) * p.run + (int)(in / (unsigned)p.nrb);
 	rb = (int)(in % (unsigned)p.nrb);
 	part = (int)(rest % (unsigned)p.ns);
-	bh = (int)(rest / (unsigned)p.ns) * p.d.Hkv + hk;
+	int b = (int)(rest / (unsigned)p.ns);
+	if (p.sort) {
+		/* the sequence with b longer ones: lane i counts those before i */
+		const int i = threadIdx.x & 63, n = i < p.d.B ? xa_len(p.d.k_len, i, p.d.Sk) : -1;
+		int before = 0;
+		for (int j = 0; j < p.d.B; ++j) {
+			const int o = __builtin_amdgcn_readlane(n, j);
+			before += o > n || (o == n && j < i);
+		}
+		b = __builtin_ctzll(__ballot(before == b && i < p.d.B));
+	}
+	bh = b * p.d.Hkv + hk;
 }
 
 /* the results of one part: for every (part, b * Hkv + h', row) DP sums,
@@ -1030,6 +1044,10 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 	a.run = 1;
 	while (d->Hkv % (2 * a.run) == 0 && 2 * a.run * d->k_h * es <= 256)
 		a.run *= 2;
+	/* 16 x 8 heads, 533 rows, lengths to 3931 of 64: 94 us, sorted 82 to 88;
+	 * two sequences gain nothing, and short ones lose to the counting (60 x 8
+	 * heads, 300 rows, to 500: 34.0 and 35.3) */
+	a.sort = parts == 1 && d->k_len && d->B > 2 && d->B <= 64 && d->Sk >= 1024 && blocks > 256;
 	int rc;
 	if (path == S3K_XATTN_MFMA) {
 		rc = d->kind == S3K_F16 ? xa_go16<S3K_F16>(a, s, (unsigned)blocks, st)

@@ -714,6 +714,20 @@ def test_cross_attention_parts(dt, B, H, Hkv, Sq, Sk, D):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
+@pytest.mark.parametrize("B,H,Hkv,Sq,D", [(3, 8, 8, 1500, 32), (17, 4, 2, 330, 64), (64, 2, 2, 260, 16), (65, 2, 2, 260, 16)])
+def test_cross_attention_many_sequences(dt, B, H, Hkv, Sq, D):
+    """Many workgroups over sequences of unlike lengths, equal ones and empty
+    ones among them, whichever is taken first."""
+    Sk = 1100
+    q, k, v = qkv(B + Sq, dt, B, H, Hkv, Sq, Sk, D)
+    g = rng(B)
+    kn = torch.randint(1, Sk + 1, (B,), generator=g).tolist()
+    kn[0], kn[1], kn[B - 1] = 0, Sk, Sk
+    check_cross(dt, q, k, v, kn=kn)
+    check_cross(dt, q, k, v, qn=[Sq - b for b in range(B)], kn=[700] * B, what="equal")
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
 @pytest.mark.parametrize("path", [0, 3])
 @pytest.mark.parametrize("Sq,Sk", [(1, 90), (1, 6000), (40, 90), (200, 2000)])
 def test_cross_attention_no_weights_over_infinite_values(dt, path, Sq, Sk):
