@@ -195,7 +195,10 @@ __global__ void __launch_bounds__(256) xa_generic(XaArgs p)
  * LDS at the end). K and V tiles of KT keys arrive by direct-to-LDS loads,
  * chunks of 16 bytes XOR-swizzled by the key, in a ring of NST stages.
  * Keys past the length and columns past D read as zeros and cost no
- * traffic.
+ * traffic. A row has DP columns in LDS and in the parts, the products go
+ * over DU of them (heads of 65 to 96: 96 of 128; 4 x 16 heads, 2000 x 2000
+ * of 80 bf16 137 us over 128, 117 over 96; f32 335 and 282 at 4 x 8 heads,
+ * 400 x 4000).
  */
 template <int DP>
 __device__ __forceinline__ int xa_kswz(int key)
@@ -228,12 +231,12 @@ struct xa_int {
 	static constexpr int value = N;
 };
 
-template <int KIND, int DP, int NWQ, int NWK, int KT, int NST>
+template <int KIND, int DP, int DU, int NWQ, int NWK, int KT, int NST>
 __global__ void __launch_bounds__(64 * NWQ * NWK, 8 / (NWQ * NWK)) xa_mfma(XaArgs p)
 {
 	/* waves that load a tile together: all, or (one wave of rows) each its own */
 	constexpr bool PRIV = NWQ == 1;
-	constexpr int LW = PRIV ? 1 : NWQ, CH = DP / 8, TB = KT * DP * 2, NMD = DP / 32, NC = DP / 16, NH = KT / 32;
+	constexpr int LW = PRIV ? 1 : NWQ, CH = DP / 8, TB = KT * DP * 2, NMD = DU / 32, NC = DU / 16, NH = KT / 32;
 	constexpr int FAM = KIND == S3K_F16 ? FAM_F16 : FAM_BF16;
 	constexpr int TI = TB / 1024, PER = TI / LW; /* 1 KiB loads: per tile, per wave */
 	static_assert(64 % CH == 0, "a load is whole rows");
@@ -497,10 +500,10 @@ constexpr int xa_f32_un(int dp)
 	return dp == 16 ? 4 : dp == 32 ? 2 : 1;
 }
 
-template <int DP, int RT, int NWQ, int NWK>
+template <int DP, int DU, int RT, int NWQ, int NWK>
 __global__ void __launch_bounds__(64 * NWQ * NWK, 2) xa_f32(XaArgs p)
 {
-	constexpr int NT = DP / 16, VW = NT < 4 ? NT : 4, NU = NT / VW;
+	constexpr int NT = DU / 16, VW = NT % 4 == 0 ? 4 : NT % 2 == 0 ? 2 : 1, NU = NT / VW;
 	constexpr int UN = xa_f32_un(DP), KT = 16 * UN, NB = DP <= 64 ? 2 : 1;
 	constexpr int MV = RT * (NT * 4 + 2); /* values a lane merges */
 	/* long heads' scores in four sums: in one after the other 256 products
@@ -893,15 +896,15 @@ XaShape xa_shape(const struct s3k_xattn *d, int path)
 	return s;
 }
 
-template <int KIND, int DP>
+template <int KIND, int DP, int DU>
 int xa_go16(const XaArgs &a, const XaShape &s, unsigned blocks, hipStream_t st)
 {
 	if (s.rows == 32) {
 		constexpr int NWK = DP == 256 ? 2 : 4, NST = DP == 32 ? 4 : 2;
-		hipLaunchKernelGGL((xa_mfma<KIND, DP, 1, NWK, 32, NST>), dim3(blocks), dim3(64 * NWK), 0, st, a);
+		hipLaunchKernelGGL((xa_mfma<KIND, DP, DU, 1, NWK, 32, NST>), dim3(blocks), dim3(64 * NWK), 0, st, a);
 	} else {
 		constexpr int KT = DP == 256 ? 32 : 64;
-		hipLaunchKernelGGL((xa_mfma<KIND, DP, 4, 1, KT, 2>), dim3(blocks), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_mfma<KIND, DP, DU, 4, 1, KT, 2>), dim3(blocks), dim3(256), 0, st, a);
 	}
 	return (int)hipGetLastError();
 }
@@ -910,20 +913,21 @@ template <int KIND>
 int xa_go16(const XaArgs &a, const XaShape &s, unsigned blocks, hipStream_t st)
 {
 	switch (s.dp) {
-	case 32: return xa_go16<KIND, 32>(a, s, blocks, st);
-	case 64: return xa_go16<KIND, 64>(a, s, blocks, st);
-	case 128: return xa_go16<KIND, 128>(a, s, blocks, st);
-	default: return xa_go16<KIND, 256>(a, s, blocks, st);
+	case 32: return xa_go16<KIND, 32, 32>(a, s, blocks, st);
+	case 64: return xa_go16<KIND, 64, 64>(a, s, blocks, st);
+	case 128:
+		return a.d.D <= 96 ? xa_go16<KIND, 128, 96>(a, s, blocks, st) : xa_go16<KIND, 128, 128>(a, s, blocks, st);
+	default: return xa_go16<KIND, 256, 256>(a, s, blocks, st);
 	}
 }
 
-template <int DP>
+template <int DP, int DU>
 int xa_gof(const XaArgs &a, const XaShape &s, unsigned blocks, hipStream_t st)
 {
 	if (s.rows == 16)
-		hipLaunchKernelGGL((xa_f32<DP, 1, 1, 4>), dim3(blocks), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_f32<DP, DU, 1, 1, 4>), dim3(blocks), dim3(256), 0, st, a);
 	else
-		hipLaunchKernelGGL((xa_f32<DP, DP == 256 ? 1 : 2, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
+		hipLaunchKernelGGL((xa_f32<DP, DU, DP == 256 ? 1 : 2, 4, 1>), dim3(blocks), dim3(256), 0, st, a);
 	return (int)hipGetLastError();
 }
 
@@ -1054,11 +1058,13 @@ extern "C" int s3k_xattn_run(const struct s3k_xattn *d, int path, int parts, voi
 					: xa_go16<S3K_BF16>(a, s, (unsigned)blocks, st);
 	} else {
 		switch (s.dp) {
-		case 16: rc = xa_gof<16>(a, s, (unsigned)blocks, st); break;
-		case 32: rc = xa_gof<32>(a, s, (unsigned)blocks, st); break;
-		case 64: rc = xa_gof<64>(a, s, (unsigned)blocks, st); break;
-		case 128: rc = xa_gof<128>(a, s, (unsigned)blocks, st); break;
-		default: rc = xa_gof<256>(a, s, (unsigned)blocks, st); break;
+		case 16: rc = xa_gof<16, 16>(a, s, (unsigned)blocks, st); break;
+		case 32: rc = xa_gof<32, 32>(a, s, (unsigned)blocks, st); break;
+		case 64: rc = xa_gof<64, 64>(a, s, (unsigned)blocks, st); break;
+		case 128:
+			rc = d->D <= 96 ? xa_gof<128, 96>(a, s, (unsigned)blocks, st) : xa_gof<128, 128>(a, s, (unsigned)blocks, st);
+			break;
+		default: rc = xa_gof<256, 256>(a, s, (unsigned)blocks, st); break;
 		}
 	}
 	if (rc != (int)hipSuccess || parts < 2)

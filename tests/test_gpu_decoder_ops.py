@@ -605,7 +605,8 @@ def qkv(seed, dt, B, H, Hkv, Sq, Sk, D, qs=1.0):
     (1, 1, 1, 1, 1, 8), (2, 4, 4, 1, 100, 64), (1, 8, 2, 1, 5000, 128), (3, 2, 1, 7, 65, 16),
     (1, 4, 1, 40, 33, 32), (2, 2, 2, 129, 200, 64), (1, 6, 2, 50, 127, 80), (1, 1, 1, 33, 64, 256),
     (1, 2, 2, 260, 1000, 128), (2, 1, 1, 200, 3000, 256), (1, 16, 4, 1, 31, 256), (1, 3, 3, 1000, 77, 32),
-    (1, 32, 1, 1, 700, 64), (1, 33, 1, 1, 300, 24), (4, 8, 8, 9, 2500, 16)])
+    (1, 32, 1, 1, 700, 64), (1, 33, 1, 1, 300, 24), (1, 2, 2, 200, 500, 72), (1, 2, 1, 40, 300, 88),
+    (1, 2, 2, 200, 300, 96), (2, 2, 1, 150, 200, 104), (1, 4, 4, 5, 90, 68), (4, 8, 8, 9, 2500, 16)])
 def test_cross_attention(dt, B, H, Hkv, Sq, Sk, D):
     q, k, v = qkv(B + H + Sq + Sk + D, dt, B, H, Hkv, Sq, Sk, D, 1.5)
     check_cross(dt, q, k, v)
@@ -701,7 +702,8 @@ def test_cross_attention_infinite_scores(dt, path):
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
 @pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [
-    (1, 1, 1, 1100, 3000, 64), (1, 2, 1, 1100, 2600, 256), (1, 1, 1, 1030, 2100, 16), (1, 1, 1, 2100, 1100, 64), (1, 4, 1, 300, 1700, 96),
+    (1, 1, 1, 1100, 3000, 64), (1, 2, 1, 1100, 2600, 256), (1, 1, 1, 1030, 2100, 16), (1, 1, 1, 2100, 1100, 64),
+    (2, 4, 2, 1, 3000, 80), (1, 1, 1, 300, 2900, 72), (1, 4, 1, 300, 1700, 96),
     (1, 1, 1, 1, 40000, 64), (1, 3, 3, 2, 9000, 24), (1, 1, 1, 1, 20001, 200)])
 def test_cross_attention_parts(dt, B, H, Hkv, Sq, Sk, D):
     """Keys shared out: many rows and few, as many parts as are ever made,
@@ -709,8 +711,8 @@ def test_cross_attention_parts(dt, B, H, Hkv, Sq, Sk, D):
     q, k, v = qkv(B + H + Sq + Sk + D, dt, B, H, Hkv, Sq, Sk, D, 1.5)
     assert hip.cross_attention_work(desc(dt, q, k, v, q)) > 0
     check_cross(dt, q, k, v)
-    check_cross(dt, q, k, v, qn=[Sq - 1], kn=[70], what="short")
-    check_cross(dt, q, k, v, kn=[0], what="none")
+    check_cross(dt, q, k, v, qn=[Sq - 1] * B, kn=[70] * B, what="short")
+    check_cross(dt, q, k, v, kn=[0] * B, what="none")
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
