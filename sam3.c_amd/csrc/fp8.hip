@@ -463,9 +463,10 @@ __device__ __forceinline__ void f8_store4(const F8Args &p, int m, int n, float4 
  * any element's address (20000 x 4001 x 500 106 us, one at a time 156): the
  * groups' pieces of two tiles are exchanged (v_permlane32_swap,
  * v_permlane16_swap) so that groups 0 and 1 hold the first tile and 2 and 3
- * the second, 64 bytes of a row together instead of 32 by halves of 8. The largest tiles' rows of whole 128-byte lines go past
- * the caches (PAST; 20736 x 4096 x 1024 114 us, through them 124); rows that
- * share lines meet there (20736 x 2000 x 1000 62, past them 83).
+ * the second, 64 bytes of a row together instead of 32 by halves of 8. The
+ * largest tiles' rows of whole 128-byte lines go past the caches (PAST;
+ * 20736 x 4096 x 1024 114 us, through them 124); rows that share lines meet
+ * there (20736 x 2000 x 1000 62, past them 83).
  */
 template <int CK, bool PAST, int NT, int MT>
 __device__ __forceinline__ void f8_tile_store(const F8Args &p, const s3k_f32x4 (&acc)[NT][MT], int m, int n,
@@ -544,9 +545,9 @@ __device__ __forceinline__ void f8_place(const F8Args &p, unsigned id, int &mt, 
  * block ahead, over the end of a tile into the next one where a workgroup
  * takes several (MANY; 20736 x 4096 x 1024 with GELU: 112 us, a workgroup
  * for each tile 117; smaller tiles, more than one on a CU, overlap by
- * themselves, and were 5 % slower with it). KS such groups of waves, each with stages of its own, take
- * every KS-th block and are added up in LDS: for few tiles, whose blocks
- * one after the other would leave most CUs idle.
+ * themselves, and were 5 % slower with it). KS such groups of waves, each
+ * with stages of its own, take every KS-th block and are added up in LDS: for
+ * few tiles, whose blocks one after the other would leave most CUs idle.
  */
 template <int CK, int BM, int BN, int WM, int WN, int KS, bool PAST>
 __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) f8_tile(F8Args p, int flags)
