@@ -454,7 +454,7 @@ enum sam3_error sam3_hip_matmul_fp8(const void *a, const float *a_scale, const v
 
 /* The whole layer: x [M, K] (F32, F16 or BF16, rows ldx elements apart)
  * quantized as sam3_hip_fp8_quantize does, then sam3_hip_matmul_fp8. Up to
- * 16 rows of at least 8 values may be quantized inside the product's
+ * 64 rows of at least 8 values may be quantized inside the product's
  * kernel (where that is quicker, or the call is captured without work
  * space): the same quantized values, sums in another order. Other calls need sam3_hip_linear_fp8_work(M, N, K) bytes for the
  * quantized copy: `work` (16-byte aligned, at least that many bytes, not

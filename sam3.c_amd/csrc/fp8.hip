@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
  * XK >= 0 (MT = 1): x of that type is quantized in registers on the way: a
  * lane holds 32 values of row lane & 15, the group's other three quarters
  * are 16, 32 and 48 lanes on. Every workgroup repeats that, which one
- * launch less pays for up to 16 rows. The last values of a K that is no
+ * launch less pays for up to 64 rows. The last values of a K that is no
  * multiple of 8 (TAIL) are read as the row's last 8 (K is at least 8) and
  * moved down; the code for it costs other lengths 0.15 to 0.5 us.
  * XK < 0: quantized rows, 16 MT of them from blockIdx.y on.
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KS, WM * WN * KS == 4 ? 2 : 1) 
 template <int XK, int CK, int MT, int NWV, bool TAIL>
 __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 {
-	static_assert(XK < 0 || MT == 1, "quantized on the way: 16 rows");
+	static_assert(XK < 0 || MT == 1, "quantized on the way: 16 rows a workgroup");
 	constexpr int RT = XK < 0 ? 1 + MT : 1, SLOT = RT * 2048; /* row tiles of a block */
 	constexpr int RED = NWV * MT * 1024, RING = NWV * 2 * SLOT;
 	__shared__ __attribute__((aligned(1024))) char smem[RED > RING ? RED : RING];
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(64 * NWV) f8_rows(F8Args p, int flags)
 			for (int c = 0; c < 4; ++c) {
 				/* bytes 16 g and 64 + 16 g onward, as the weights' */
 				const int k = k0 + 64 * (c >> 1) + 8 * (c & 1);
-				x[S][c] = f8_chunk<XK>(p.x, l16 * p.ldx + (TAIL ? min(k, p.K - 8) : k), l16 < p.M && k < p.K);
+				x[S][c] = f8_chunk<XK>(p.x, (m0 + l16) * p.ldx + (TAIL ? min(k, p.K - 8) : k), m0 + l16 < p.M && k < p.K);
 			}
 		}
 	};

@@ -445,7 +445,7 @@ int s3k_fp8_matmul(const void *q, const float *sa, const void *w, const float *s
 		   void *c, int M, int N, int K, const void *bias, int flags, void *stream);
 /* x of up to S3K_FP8_ROWS_MAX rows, quantized inside the product's kernel,
  * where s3k_fp8_rows_ok (K of 8 at least, or 0) */
-#define S3K_FP8_ROWS_MAX 16
+#define S3K_FP8_ROWS_MAX 64
 int s3k_fp8_rows_ok(int M, int K);
 int s3k_fp8_rows(int xk, const void *x, long long ldx, const void *w, const float *sw, int ck,
 		 void *c, int M, int N, int K, const void *bias, int flags, void *stream);

@@ -164,11 +164,14 @@ enum sam3_error sam3_hip_linear_fp8(int x_dtype, const void *x, long long ldx, c
 		return SAM3_OK;
 	if (K > 0 && (!x || (uintptr_t)x % esize(x_dtype)))
 		REFUSE(SAM3_EINVAL, "linear_fp8: x is NULL or not element-aligned");
-	/* Every workgroup quantizes all of x again: with more than 256 blocks of
-	 * it a launch of its own is quicker (16 x 4096 x 4096 6.7 us, inside 7.8;
-	 * 8 x 4096 x 4096 6.4 and 6.3; 16 x 1024 x 1024 5.2 and 3.6). */
-	if (s3k_fp8_rows_ok(M, K) &&
-	    ((long long)M * ((K + 127) / 128) <= 256 || (!work && captured(stream))))
+	/* Every workgroup quantizes its 16 rows of x again: with more than 256
+	 * blocks of x a launch of its own is quicker (16 x 4096 x 4096 6.7 us,
+	 * inside 7.8; 8 x 4096 x 4096 6.4 and 6.3; 64 x 1024 x 512 4.9 and 3.2), and
+	 * with many workgroups for more than 16 rows (64 x 8192 x 512 6.7 and 8.0;
+	 * 64 x 4096 x 512 6.3 and 5.2). */
+	const long long wgs = ((N + 15ll) / 16) * ((M + 15ll) / 16);
+	const int inside = (long long)M * ((K + 127) / 128) <= 256 && (M <= 16 || wgs <= 1024);
+	if (s3k_fp8_rows_ok(M, K) && (inside || (!work && captured(stream))))
 		return launched(s3k_fp8_rows(x_dtype, x, ldx, w, w_scale, c_dtype, c, M, N, K, bias, flags,
 					    stream),
 			       "linear_fp8");

@@ -331,7 +331,7 @@ def test_linear_fp8(dt, M, N, K, pad, flags):
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS.get)
-@pytest.mark.parametrize("M,pad", [(1, 0), (16, 1), (5, 3)])
+@pytest.mark.parametrize("M,pad", [(1, 0), (16, 1), (5, 3), (17, 0), (33, 5), (64, 1), (65, 0)])
 @pytest.mark.parametrize("K", [1, 7, 8, 9, 12, 15, 23, 127, 129, 135, 250, 1029, 4097])
 def test_linear_fp8_few_rows_of_any_length(dt, M, pad, K):
     """Few rows whose last values fill no eight of them, at odd addresses,
@@ -385,7 +385,7 @@ def test_linear_fp8_captured(env):
     replayed; without it a call that needs some is refused."""
     env.set("SAM3_HIP_QUIET", "1")
     g = rng(4)
-    for M, N, K in ((3, 300, 520), (90, 300, 520), (16, 100, 4104), (5, 100, 515), (5, 100, 7)):
+    for M, N, K in ((3, 300, 520), (90, 300, 520), (50, 200, 2001), (16, 100, 4104), (5, 100, 515), (5, 100, 7)):
         w8, sw = (t.cuda() for t in weights(g, N, K))
         xs = [torch.randn(M, K, generator=g).cuda() for _ in range(3)]
         x, c = xs[0].clone(), torch.empty(M, N, device="cuda")
@@ -396,7 +396,7 @@ def test_linear_fp8_captured(env):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             st = stream()
-            if M > 16 or K < 8:
+            if M > 64 or K < 8:
                 with pytest.raises(hip.HipError):
                     hip.linear_fp8_dev(abi.F32, x.data_ptr(), w8.data_ptr(), sw.data_ptr(), abi.F32,
                                        c.data_ptr(), M, N, K, stream=st)
